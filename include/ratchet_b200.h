@@ -42,6 +42,7 @@ extern "C" {
 #define RT_STATUS_PRESSURE_RANGE 0x8u     /* validate: |pressure| > 7                            */
 #define RT_STATUS_SCALE_INVALID 0x10u     /* validate: a row scale is <= 0 or non-finite         */
 #define RT_STATUS_INDEX_RANGE 0x20u       /* a token id / window outside its table (zeros used)  */
+#define RT_STATUS_NONFINITE_KV 0x40u      /* rt_kv_append met NaN/Inf (stored as 0 / the largest code) */
 
 int rt_abi_version(void);
 const char *rt_last_error(void);
@@ -367,6 +368,59 @@ int rt_embedding_ratchet_update(const float *grad, int64_t ldg, const int64_t *s
                                 void *stream);
 int rt_token_windows(const uint16_t *data, int64_t n, const int64_t *starts, int64_t batch,
                      int64_t block, int64_t *inputs, int64_t *targets, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Paged int8 key/value cache (no counterpart in the reference, whose generate.py:137 runs the whole
+ * window again for every token).  One layer's cache:
+ *   codes  int8 [n_pages, 2 (K|V), kv_heads, page_size, padded_dim], contiguous, 16-byte aligned
+ *   scales fp32 [n_pages, 2, kv_heads, page_size / 16]: value = code * scale of its 16-token block
+ * page_size is 16, 32, 64, 128 or 256; padded_dim is 32, 64, 128 or 256, the head width rounded up
+ * (codes beyond head_dim are zero).  A batch, all of it read on the device:
+ *   page_table int32 [n_seqs, pages_per_seq]: page of tokens [i * page_size, (i + 1) * page_size)
+ *   kv_lens int32 [n_seqs]: tokens of each sequence, the newest ones of this call included
+ *   cu_tokens int32 [n_seqs + 1]: rows [cu[s], cu[s + 1]) of the call are sequence s's newest tokens,
+ *     at its last positions; cu[0] = 0.  Rows from cu[n_seqs] to n_tokens belong to no sequence
+ *     (append ignores them, read and attention write zeros).
+ * Lengths, rows or pages outside their bounds are cut to them, never followed, and set
+ * RT_STATUS_INDEX_RANGE.
+ *
+ * rt_kv_append: stores the newest tokens' k and v (fp32 or bf16, [n_tokens, kv_heads, head_dim] with
+ *   the given element strides, unit innermost).  Per 16-token block, with p0 the first new row:
+ *   old = p0 > 0 ? scale : 0; s = max(old, max|new| / 127, FLT_MIN); held codes become
+ *   rint(code * (old / s)) when s > old; new codes are clamp(rint(x / s), -127, 127).  A sequence
+ *   may appear once in a batch, and no two sequences may append into one page.
+ * rt_kv_read: k_out, v_out [n_tokens, kv_heads, head_dim] contiguous = code * scale (one rounding to
+ *   dtype) at positions starts[s] + i of row cu[s] + i.
+ * rt_kv_copy_pages: copies pages src[i] -> dst[i] (device int32 [n]) of codes [layers, n_pages, ...]
+ *   and scales over all layers, and, with table_entries > 0, replaces every page_table entry equal
+ *   to src[i] by dst[i].  No page may be both a source and a destination, or a destination twice.
+ * rt_kv_attention: out[t, h] = softmax over the keys at positions <= row t's own of
+ *   softmax_scale * (q[t, h] . k), times v; query head h reads kv head h / (q_heads / kv_heads).
+ *   A row that sees no key is zero.  Scores, maxima, sums and outputs are fp32, rounded once to dtype.
+ *   workspace: rt_kv_attention_workspace_bytes(...) bytes, 256-byte aligned, no initial contents.
+ * ------------------------------------------------------------------------------------------- */
+int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t kv_heads, int64_t page_size,
+                 int64_t padded_dim, const int32_t *page_table, int64_t pages_per_seq,
+                 const int32_t *kv_lens, const int32_t *cu_tokens, int64_t n_seqs, int64_t n_tokens,
+                 const void *k, const void *v, int dtype, int64_t head_dim, int64_t k_stride_token,
+                 int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head, void *stream);
+int rt_kv_read(const void *codes, const float *scales, int64_t n_pages, int64_t kv_heads,
+               int64_t page_size, int64_t padded_dim, const int32_t *page_table,
+               int64_t pages_per_seq, const int32_t *starts, const int32_t *cu_tokens,
+               int64_t n_seqs, int64_t n_tokens, int64_t head_dim, void *k_out, void *v_out,
+               int dtype, void *stream);
+int rt_kv_copy_pages(void *codes, float *scales, int64_t layers, int64_t n_pages, int64_t kv_heads,
+                     int64_t page_size, int64_t padded_dim, const int32_t *src, const int32_t *dst,
+                     int64_t n, int32_t *page_table, int64_t table_entries, void *stream);
+int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token, int64_t q_stride_head,
+                    int64_t q_heads, int64_t head_dim, const void *codes, const float *scales,
+                    int64_t n_pages, int64_t kv_heads, int64_t page_size, int64_t padded_dim,
+                    const int32_t *page_table, int64_t pages_per_seq, const int32_t *kv_lens,
+                    const int32_t *cu_tokens, int64_t n_seqs, int64_t n_tokens, double softmax_scale,
+                    void *out, int64_t o_stride_token, int64_t o_stride_head, void *workspace,
+                    int64_t workspace_bytes, void *stream);
+int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
+                                        int64_t kv_heads, int64_t padded_dim);
 
 #ifdef __cplusplus
 }

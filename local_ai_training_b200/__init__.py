@@ -10,6 +10,7 @@ from .int8_matmul import (
     quantize_rows_colscaled,
     scaled_int8_mm,
 )
+from .kv_cache import PagedKVCache, kv_append, kv_attention, kv_copy_pages, kv_read
 from .model import ModelConfig, RatchetGPT, build_seeded_model
 from .ratchet import (
     DiscreteRatchetLinear,
@@ -27,6 +28,7 @@ from .ratchet import (
 __all__ = [
     "DiscreteRatchetLinear",
     "ModelConfig",
+    "PagedKVCache",
     "PersistentFootprint",
     "RatchetAuditReport",
     "RatchetEmbedding",
@@ -36,6 +38,10 @@ __all__ = [
     "bucket_pressure",
     "build_seeded_model",
     "compare_persistent_footprint",
+    "kv_append",
+    "kv_attention",
+    "kv_copy_pages",
+    "kv_read",
     "pack_code_pressure",
     "quantize_columns",
     "quantize_rows",

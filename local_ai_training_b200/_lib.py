@@ -23,6 +23,7 @@ STATUS_CODE_RANGE = 0x4
 STATUS_PRESSURE_RANGE = 0x8
 STATUS_SCALE_INVALID = 0x10
 STATUS_INDEX_RANGE = 0x20
+STATUS_NONFINITE_KV = 0x40
 
 _ERR_INVALID, _ERR_DTYPE, _ERR_ALIGN = 1, 2, 3
 ABI_VERSION = 2
@@ -87,6 +88,14 @@ _SIGNATURES = {
     "rt_cross_entropy_fwd": ([_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p], _i),
     "rt_cross_entropy_bwd": ([_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _p,
                               _i64, _p], _i),
+    "rt_kv_append": ([_p, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _i, _i64,
+                      _i64, _i64, _i64, _i64, _p], _i),
+    "rt_kv_read": ([_p, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i,
+                    _p], _i),
+    "rt_kv_copy_pages": ([_p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p], _i),
+    "rt_kv_attention": ([_p, _i, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i64,
+                         _p, _p, _i64, _i64, _d, _p, _i64, _i64, _p, _i64, _p], _i),
+    "rt_kv_attention_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
 }
 
 

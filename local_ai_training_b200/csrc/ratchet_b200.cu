@@ -4,3 +4,4 @@
 #include "rt_rowops.cuh"
 #include "rt_gemm.cuh"
 #include "rt_loss.cuh"
+#include "rt_cache.cuh"

@@ -1,0 +1,481 @@
+// rt_cache.cuh — paged int8 key/value cache: append, read back, page copies and causal attention.
+//
+// One layer's cache is codes int8 [pages, 2 (K|V), kv_heads, page_size, padded_dim] and scales fp32
+// [pages, 2, kv_heads, page_size / 16]: the value of a code is code · scale of its block of 16 tokens.
+// A page of one head is contiguous (page_size · padded_dim bytes), so a 16-token block is one
+// contiguous piece too.  A batch is a page table [seqs, pages_per_seq], the sequences' lengths with
+// their newest tokens (kv_lens) and the prefix sums of the newest tokens (cu_tokens [seqs + 1]).
+// All of it lives on the device; nothing here reads it on the host, so a captured graph can be
+// replayed while lengths and tables change.
+#pragma once
+
+#include "rt_common.cuh"
+
+namespace rt {
+
+constexpr int KV_BLOCK = 16;  // tokens that share a scale
+
+struct KvCache {
+  int8_t *codes;
+  float *scales;
+  int64_t n_pages;
+  int kv_heads, page_size, page_shift, dim;  // dim: padded head width
+  // bytes of one page and floats of its scales
+  __host__ __device__ int64_t page_bytes() const {
+    return static_cast<int64_t>(2) * kv_heads * page_size * dim;
+  }
+  // block `blk` (of 16 tokens) of a page, part 0 = K, 1 = V
+  __device__ int8_t *block(int64_t page, int part, int head, int blk) const {
+    return codes + (((page * 2 + part) * kv_heads + head) * page_size + blk * KV_BLOCK) * dim;
+  }
+  __device__ float *scale(int64_t page, int part, int head, int blk) const {
+    return scales + ((page * 2 + part) * kv_heads + head) * (page_size / KV_BLOCK) + blk;
+  }
+};
+
+struct KvBatch {
+  const int32_t *page_table;
+  int64_t pages_per_seq;
+  const int32_t *kv_lens;
+  const int32_t *cu;
+  int64_t n_seqs, n_tokens;
+};
+
+// Newest tokens of sequence s: rows [c0, c0 + n) at positions [start, start + n), start = len - n.
+// Values outside the batch's own bounds are cut to them and flagged.
+struct KvSeq {
+  int c0, n, len, start;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvBatch &b, int page_size, int64_t s) {
+  const int t = static_cast<int>(b.n_tokens);
+  const int c0 = b.cu[s], c1 = b.cu[s + 1], len = b.kv_lens[s];
+  const int64_t room = b.pages_per_seq * page_size;
+  KvSeq q;
+  q.c0 = min(max(c0, 0), t);
+  q.n = max(min(max(c1, 0), t) - q.c0, 0);
+  q.len = static_cast<int>(min(static_cast<int64_t>(max(len, 0)), room));
+  q.start = q.len - q.n;
+  if (q.c0 != c0 || q.c0 + q.n != c1 || q.len != len || q.start < 0)
+    raise_status(RT_STATUS_INDEX_RANGE);
+  return q;
+}
+// Page that holds block `blk` of sequence s, or -1 (flagged) when the table names none.
+__device__ __forceinline__ int64_t kv_page(const KvCache &c, const KvBatch &b, int64_t s, int blk) {
+  const int32_t p = __ldg(b.page_table + s * b.pages_per_seq + (blk >> (c.page_shift - 4)));
+  if (p < 0 || p >= c.n_pages) {
+    raise_status(RT_STATUS_INDEX_RANGE);
+    return -1;
+  }
+  return p;
+}
+// The sequence whose rows hold row t (cu[s] <= t < cu[s + 1]), or -1.
+__device__ __forceinline__ int64_t kv_seq_of(const int32_t *cu, int64_t n_seqs, int64_t t) {
+  int64_t lo = 0, hi = n_seqs;  // first s with cu[s + 1] > t
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (__ldg(cu + mid + 1) > t)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo < n_seqs && __ldg(cu + lo) <= t ? lo : -1;
+}
+
+// ------------------------------------------------------------------------------------------
+// Append.  Per touched block of 16 tokens (new rows from row p0 on; rows before p0 were held):
+//   old = p0 > 0 ? scale : 0,  s = max(old, RN(max|new| / 127), FLT_MIN)
+//   held rows, when s > old:  q = rint(q · RN(old / s));   new rows:  q = clamp(rint(RN(x / s)))
+// One warp per (block, K|V, head): the block's scale has one writer.  A non-finite x takes no part in
+// the maximum, is stored as 0 (NaN) or ±127 (infinity) and is flagged.
+// Slots: sequence s owns slots [cu[s] / 16 + 2s, cu[s + 1] / 16 + 2(s + 1)), at least as many as the
+// blocks its n tokens can touch (n / 16 + 2), so no prefix sum over the batch is needed.
+// ------------------------------------------------------------------------------------------
+struct KvNew {
+  const void *k, *v;
+  int64_t k_token, k_head, v_token, v_head;  // element strides
+  int head_dim;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int per = 2 * c.kv_heads;
+  const int slot = static_cast<int>(w / per), part = static_cast<int>(w % per) / c.kv_heads;
+  const int head = static_cast<int>(w % c.kv_heads);
+  if (slot >= slots) return;
+  int64_t lo = 0, hi = b.n_seqs;  // last s whose first slot is <= slot
+  while (lo + 1 < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if ((max(__ldg(b.cu + mid), 0) >> 4) + 2 * mid <= slot)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const KvSeq q = kv_seq(b, c.page_size, lo);
+  if (q.n == 0) return;
+  const int blk = (max(q.start, 0) >> 4) + slot - ((q.c0 >> 4) + 2 * static_cast<int>(lo));
+  if (blk * KV_BLOCK >= q.len || blk < 0) return;
+  const int64_t page = kv_page(c, b, lo, blk);
+  if (page < 0) return;
+  const int in_page = blk & ((c.page_size >> 4) - 1);
+  int8_t *dst = c.block(page, part, head, in_page);
+  float *sp = c.scale(page, part, head, in_page);
+  const int p0 = max(q.start - blk * KV_BLOCK, 0);            // first new row
+  const int p1 = min(q.len - blk * KV_BLOCK, KV_BLOCK);       // rows of the block in use
+  const int64_t st = part == 0 ? x.k_token : x.v_token, sh = part == 0 ? x.k_head : x.v_head;
+  const T *src = static_cast<const T *>(part == 0 ? x.k : x.v) +
+                 (q.c0 + static_cast<int64_t>(blk) * KV_BLOCK - q.start) * st + head * sh;
+  float amax = 0.0f;
+  bool odd = false;
+  for (int r = p0; r < p1; ++r)
+    for (int d = lane; d < x.head_dim; d += 32) {
+      const float a = fabsf(load_as_float(src + r * st + d));
+      if (a <= FLT_MAX)
+        amax = fmaxf(amax, a);
+      else
+        odd = true;
+    }
+  amax = warp_max(amax);
+  if (odd) raise_status(RT_STATUS_NONFINITE_KV);
+  const float old = p0 > 0 ? *sp : 0.0f;
+  const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
+  if (p0 > 0 && s > old) {
+    const float ratio = __fdiv_rn(old, s);
+    for (int i = lane; i < p0 * c.dim; i += 32)
+      dst[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(dst[i]), ratio)));
+  }
+  for (int r = p0; r < p1; ++r)
+    for (int d = lane; d < c.dim; d += 32) {
+      float q8 = 0.0f;
+      if (d < x.head_dim) {
+        const float v = load_as_float(src + r * st + d);
+        q8 = v != v ? 0.0f : fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
+      }
+      dst[r * c.dim + d] = static_cast<int8_t>(static_cast<int>(q8));
+    }
+  __syncwarp();
+  if (lane == 0) *sp = s;
+}
+
+// ------------------------------------------------------------------------------------------
+// Read back: out[t, h, d] = round(float(code) · scale) for positions starts[s] + i of each sequence.
+// ------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void store_from_float(T *p, float v);
+template <>
+__device__ __forceinline__ void store_from_float<float>(float *p, float v) { *p = v; }
+template <>
+__device__ __forceinline__ void store_from_float<__nv_bfloat16>(__nv_bfloat16 *p, float v) {
+  *p = __float2bfloat16_rn(v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    kv_read_kernel(KvCache c, KvBatch b, int head_dim, T *k_out, T *v_out) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t t = blockIdx.x;
+  const int64_t s = kv_seq_of(b.cu, b.n_seqs, t);
+  const int64_t pos = s < 0 ? -1 : __ldg(b.kv_lens + s) + t - __ldg(b.cu + s);
+  const bool in = pos >= 0 && pos < b.pages_per_seq * c.page_size;
+  if (s >= 0 && !in) raise_status(RT_STATUS_INDEX_RANGE);
+  const int64_t page = in ? kv_page(c, b, s, static_cast<int>(pos >> 4)) : -1;
+  const int row = static_cast<int>(pos & 15), blk = static_cast<int>(pos >> 4) & ((c.page_size >> 4) - 1);
+  const int n = c.kv_heads * head_dim;
+  for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
+    const int part = i >= n, j = i - part * n, h = j / head_dim, d = j % head_dim;
+    float v = 0.0f;
+    if (page >= 0)
+      v = __fmul_rn(static_cast<float>(c.block(page, part, h, blk)[row * c.dim + d]),
+                    *c.scale(page, part, h, blk));
+    store_from_float((part ? v_out : k_out) + t * n + j, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Page copies over all layers, and the page table's entries rewritten from src to dst.
+// ------------------------------------------------------------------------------------------
+struct KvCopy {
+  int8_t *codes;
+  float *scales;
+  int64_t layers, n_pages, page_bytes, page_scales;
+  const int32_t *src, *dst;
+  int n;
+  int32_t *table;
+  int64_t entries;
+};
+
+__global__ void __launch_bounds__(256) kv_copy_kernel(KvCopy a, int copy_blocks) {
+  pdl_wait();
+  pdl_trigger();
+  if (static_cast<int>(blockIdx.x) >= copy_blocks) {  // the table's share of the grid
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) - copy_blocks) * blockDim.x + threadIdx.x;
+    if (at >= a.entries) return;
+    const int32_t p = a.table[at];
+    for (int i = 0; i < a.n; ++i)
+      if (__ldg(a.src + i) == p) {
+        a.table[at] = __ldg(a.dst + i);
+        break;
+      }
+    return;
+  }
+  const int64_t pair = blockIdx.x % a.n, layer = blockIdx.x / a.n;
+  const int32_t s = __ldg(a.src + pair), d = __ldg(a.dst + pair);
+  if (s < 0 || s >= a.n_pages || d < 0 || d >= a.n_pages) {
+    raise_status(RT_STATUS_INDEX_RANGE);
+    return;
+  }
+  const int4 *from = reinterpret_cast<const int4 *>(a.codes + (layer * a.n_pages + s) * a.page_bytes);
+  int4 *to = reinterpret_cast<int4 *>(a.codes + (layer * a.n_pages + d) * a.page_bytes);
+  for (int64_t i = threadIdx.x; i < a.page_bytes / 16; i += blockDim.x) to[i] = from[i];
+  const float *sf = a.scales + (layer * a.n_pages + s) * a.page_scales;
+  float *st = a.scales + (layer * a.n_pages + d) * a.page_scales;
+  for (int64_t i = threadIdx.x; i < a.page_scales; i += blockDim.x) st[i] = sf[i];
+}
+
+// ------------------------------------------------------------------------------------------
+// Causal attention of the newest tokens over the cache: query row i of a sequence sits at position
+// start + i and sees the keys at positions <= its own.
+//   o = sum_j exp2(t_j - m) · sv_j · V_j / sum_j exp2(t_j - m),  t_j = scale · log2(e) · sk_j · (q · K_j)
+// A row that sees no key is zero, as is a row of no sequence.
+// ------------------------------------------------------------------------------------------
+struct KvAttn {
+  const void *q;
+  int64_t q_token, q_head;
+  void *out;
+  int64_t o_token, o_head;
+  int q_heads, head_dim;
+  float scale_log2;  // softmax scale · log2(e)
+};
+
+// One warp per (row, query head); lanes over the head's width.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_attention_row_kernel(KvCache c, KvBatch b, KvAttn a) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t t = w / a.q_heads;
+  const int h = static_cast<int>(w % a.q_heads), kvh = h / (a.q_heads / c.kv_heads);
+  if (t >= b.n_tokens) return;
+  const T *q = static_cast<const T *>(a.q) + t * a.q_token + h * a.q_head;
+  T *o = static_cast<T *>(a.out) + t * a.o_token + h * a.o_head;
+  float qv[8], acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    qv[i] = d < a.head_dim ? load_as_float(q + d) : 0.0f;
+    acc[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  const int64_t s = kv_seq_of(b.cu, b.n_seqs, t);
+  int seen = 0;
+  if (s >= 0) {
+    const KvSeq sq = kv_seq(b, c.page_size, s);
+    seen = min(sq.start + static_cast<int>(t) - sq.c0 + 1, sq.len);
+  }
+  for (int blk = 0; blk * KV_BLOCK < seen; ++blk) {
+    const int64_t page = kv_page(c, b, s, blk);
+    if (page < 0) continue;
+    const int in_page = blk & ((c.page_size >> 4) - 1);
+    const int8_t *kp = c.block(page, 0, kvh, in_page), *vp = c.block(page, 1, kvh, in_page);
+    const float sk = *c.scale(page, 0, kvh, in_page) * a.scale_log2;
+    const float sv = *c.scale(page, 1, kvh, in_page);
+    const int rows = min(KV_BLOCK, seen - blk * KV_BLOCK);
+    for (int r = 0; r < rows; ++r) {
+      float dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < c.dim) dot += qv[i] * static_cast<float>(kp[r * c.dim + lane + 32 * i]);
+      const float x = warp_sum_butterfly(dot) * sk;
+      const float mn = fmaxf(m, x), f = exp2f(m - mn), p = exp2f(x - mn);
+      l = l * f + p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < c.dim)
+          acc[i] = acc[i] * f + p * sv * static_cast<float>(vp[r * c.dim + lane + 32 * i]);
+      m = mn;
+    }
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = lane + 32 * i;
+    if (d < a.head_dim) store_from_float(o + d, acc[i] * inv);
+  }
+}
+
+// Shared argument checks of the cache entry points; 0 or the failure's status.
+inline int kv_check(const char *what, const void *codes, const void *scales, int64_t n_pages,
+                    int64_t kv_heads, int64_t page_size, int64_t dim, int64_t head_dim,
+                    KvCache *c) {
+  if (n_pages <= 0 || kv_heads <= 0 || n_pages > INT32_MAX || kv_heads > 65535)
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: cache shape", what);
+  if (page_size < KV_BLOCK || page_size > 256 || (page_size & (page_size - 1)) != 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: page_size must be 16, 32, 64, 128 or 256", what);
+  if (dim != 32 && dim != 64 && dim != 128 && dim != 256)
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: padded head width must be 32, 64, 128 or 256", what);
+  if (head_dim <= 0 || head_dim > dim)
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: head_dim must be in [1, padded head width]", what);
+  if (codes == nullptr || scales == nullptr)
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (!aligned16(codes)) return fail(RT_ERR_ALIGNMENT, "%s: codes must be 16-byte aligned", what);
+  c->codes = static_cast<int8_t *>(const_cast<void *>(codes));
+  c->scales = static_cast<float *>(const_cast<void *>(scales));
+  c->n_pages = n_pages, c->kv_heads = static_cast<int>(kv_heads);
+  c->page_size = static_cast<int>(page_size), c->dim = static_cast<int>(dim);
+  c->page_shift = 4;
+  while ((1 << c->page_shift) < page_size) ++c->page_shift;
+  return RT_OK;
+}
+inline int kv_check_batch(const char *what, const int32_t *page_table, int64_t pages_per_seq,
+                          const int32_t *lens, const int32_t *cu, int64_t n_seqs, int64_t n_tokens,
+                          int64_t page_size, KvBatch *b) {
+  if (n_seqs < 0 || n_tokens < 0 || pages_per_seq < 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: negative shape", what);
+  if (n_seqs > (1 << 20) || n_tokens > (1 << 30) || pages_per_seq * page_size > (1ll << 30))
+    return fail(RT_ERR_UNSUPPORTED, "%s: batch too large", what);
+  if (n_seqs > 0 && (lens == nullptr || cu == nullptr || (page_table == nullptr && pages_per_seq > 0)))
+    return fail(RT_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  *b = KvBatch{page_table, pages_per_seq, lens, cu, n_seqs, n_tokens};
+  return RT_OK;
+}
+
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t kv_heads,
+                            int64_t page_size, int64_t padded_dim, const int32_t *page_table,
+                            int64_t pages_per_seq, const int32_t *kv_lens, const int32_t *cu_tokens,
+                            int64_t n_seqs, int64_t n_tokens, const void *k, const void *v, int dtype,
+                            int64_t head_dim, int64_t k_stride_token, int64_t k_stride_head,
+                            int64_t v_stride_token, int64_t v_stride_head, void *stream) {
+  KvCache c;
+  KvBatch b;
+  if (int rc = kv_check("kv_append", codes, scales, n_pages, kv_heads, page_size, padded_dim,
+                        head_dim, &c))
+    return rc;
+  if (int rc = kv_check_batch("kv_append", page_table, pages_per_seq, kv_lens, cu_tokens, n_seqs,
+                              n_tokens, page_size, &b))
+    return rc;
+  if (dtype != RT_F32 && dtype != RT_BF16)
+    return fail(RT_ERR_DTYPE, "kv_append: keys and values must be float32 or bfloat16");
+  if (n_tokens == 0 || n_seqs == 0) return RT_OK;
+  if (k == nullptr || v == nullptr) return fail(RT_ERR_INVALID_ARGUMENT, "kv_append: null pointer");
+  const KvNew x{k, v, k_stride_token, k_stride_head, v_stride_token, v_stride_head,
+                static_cast<int>(head_dim)};
+  const int64_t slots = n_tokens / KV_BLOCK + 2 * n_seqs;
+  const int64_t grid = (slots * 2 * kv_heads + 7) / 8;
+  if (grid > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "kv_append: batch too large");
+  cudaStream_t s = as_stream(stream);
+  if (dtype == RT_F32)
+    launch_k(kv_append_kernel<float>, static_cast<unsigned>(grid), 256, 0, s, c, b, x,
+             static_cast<int>(slots));
+  else
+    launch_k(kv_append_kernel<__nv_bfloat16>, static_cast<unsigned>(grid), 256, 0, s, c, b, x,
+             static_cast<int>(slots));
+  return check_launch("kv_append");
+}
+
+extern "C" int rt_kv_read(const void *codes, const float *scales, int64_t n_pages, int64_t kv_heads,
+                          int64_t page_size, int64_t padded_dim, const int32_t *page_table,
+                          int64_t pages_per_seq, const int32_t *starts, const int32_t *cu_tokens,
+                          int64_t n_seqs, int64_t n_tokens, int64_t head_dim, void *k_out,
+                          void *v_out, int dtype, void *stream) {
+  KvCache c;
+  KvBatch b;
+  if (int rc = kv_check("kv_read", codes, scales, n_pages, kv_heads, page_size, padded_dim, head_dim,
+                        &c))
+    return rc;
+  if (int rc = kv_check_batch("kv_read", page_table, pages_per_seq, starts, cu_tokens, n_seqs,
+                              n_tokens, page_size, &b))
+    return rc;
+  if (dtype != RT_F32 && dtype != RT_BF16)
+    return fail(RT_ERR_DTYPE, "kv_read: output must be float32 or bfloat16");
+  if (n_tokens == 0) return RT_OK;
+  if (k_out == nullptr || v_out == nullptr)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_read: null pointer");
+  cudaStream_t s = as_stream(stream);
+  const unsigned grid = static_cast<unsigned>(n_tokens);
+  if (dtype == RT_F32)
+    launch_k(kv_read_kernel<float>, grid, 256, 0, s, c, b, static_cast<int>(head_dim),
+             static_cast<float *>(k_out), static_cast<float *>(v_out));
+  else
+    launch_k(kv_read_kernel<__nv_bfloat16>, grid, 256, 0, s, c, b, static_cast<int>(head_dim),
+             static_cast<__nv_bfloat16 *>(k_out), static_cast<__nv_bfloat16 *>(v_out));
+  return check_launch("kv_read");
+}
+
+extern "C" int rt_kv_copy_pages(void *codes, float *scales, int64_t layers, int64_t n_pages,
+                                int64_t kv_heads, int64_t page_size, int64_t padded_dim,
+                                const int32_t *src, const int32_t *dst, int64_t n,
+                                int32_t *page_table, int64_t table_entries, void *stream) {
+  KvCache c;
+  if (int rc = kv_check("kv_copy_pages", codes, scales, n_pages, kv_heads, page_size, padded_dim, 1,
+                        &c))
+    return rc;
+  if (layers <= 0 || n < 0 || table_entries < 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_copy_pages: negative shape");
+  if (n == 0) return RT_OK;
+  if (src == nullptr || dst == nullptr || (page_table == nullptr && table_entries > 0))
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_copy_pages: null pointer");
+  const int64_t blocks = n * layers, table_blocks = (table_entries + 255) / 256;
+  if (n > n_pages || blocks + table_blocks > INT32_MAX)
+    return fail(RT_ERR_UNSUPPORTED, "kv_copy_pages: more pairs than pages");
+  KvCopy a{c.codes, c.scales, layers, n_pages, c.page_bytes(),
+           2 * kv_heads * (page_size / KV_BLOCK), src, dst, static_cast<int>(n), page_table,
+           table_entries};
+  launch_k(kv_copy_kernel, static_cast<unsigned>(blocks + table_blocks), 256, 0, as_stream(stream),
+           a, static_cast<int>(blocks));
+  return check_launch("kv_copy_pages");
+}
+
+extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
+                                                   int64_t kv_heads, int64_t padded_dim) {
+  (void)n_seqs, (void)n_tokens, (void)q_heads, (void)kv_heads, (void)padded_dim;
+  return 0;
+}
+
+extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
+                               int64_t q_stride_head, int64_t q_heads, int64_t head_dim,
+                               const void *codes, const float *scales, int64_t n_pages,
+                               int64_t kv_heads, int64_t page_size, int64_t padded_dim,
+                               const int32_t *page_table, int64_t pages_per_seq,
+                               const int32_t *kv_lens, const int32_t *cu_tokens, int64_t n_seqs,
+                               int64_t n_tokens, double softmax_scale, void *out,
+                               int64_t o_stride_token, int64_t o_stride_head, void *workspace,
+                               int64_t workspace_bytes, void *stream) {
+  KvCache c;
+  KvBatch b;
+  if (int rc = kv_check("kv_attention", codes, scales, n_pages, kv_heads, page_size, padded_dim,
+                        head_dim, &c))
+    return rc;
+  if (int rc = kv_check_batch("kv_attention", page_table, pages_per_seq, kv_lens, cu_tokens, n_seqs,
+                              n_tokens, page_size, &b))
+    return rc;
+  if (dtype != RT_F32 && dtype != RT_BF16)
+    return fail(RT_ERR_DTYPE, "kv_attention: queries must be float32 or bfloat16");
+  if (q_heads <= 0 || q_heads % kv_heads != 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: query heads must be a multiple of kv heads");
+  if (!(softmax_scale == softmax_scale) || softmax_scale - softmax_scale != 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: softmax scale must be finite");
+  if (n_tokens == 0) return RT_OK;
+  if (q == nullptr || out == nullptr)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: null pointer");
+  (void)workspace, (void)workspace_bytes;
+  const KvAttn a{q, q_stride_token, q_stride_head, out, o_stride_token, o_stride_head,
+                 static_cast<int>(q_heads), static_cast<int>(head_dim),
+                 static_cast<float>(softmax_scale * 1.4426950408889634)};
+  const int64_t grid = (n_tokens * q_heads + 7) / 8;
+  if (grid > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
+  cudaStream_t s = as_stream(stream);
+  if (dtype == RT_F32)
+    launch_k(kv_attention_row_kernel<float>, static_cast<unsigned>(grid), 256, 0, s, c, b, a);
+  else
+    launch_k(kv_attention_row_kernel<__nv_bfloat16>, static_cast<unsigned>(grid), 256, 0, s, c, b, a);
+  return check_launch("kv_attention");
+}

@@ -1,0 +1,408 @@
+"""Paged int8 key/value cache: append, attention, read back and page copies on sm_100a.
+
+The reference's generation (generate.py:137) runs the whole window again for every token; here the
+keys and values of earlier tokens stay on the device as int8 codes with one fp32 scale for each block
+of 16 tokens, head and K|V, in pages that sequences share and copy on write.
+
+Tensors of one layer: codes int8 [pages, 2 (K|V), kv_heads, page_size, padded head width], scales
+fp32 [pages, 2, kv_heads, page_size / 16].  A batch: page_table int32 [seqs, pages per sequence],
+kv_lens int32 [seqs] (tokens with the newest ones), cu_tokens int32 [seqs + 1] (prefix sums of the
+newest tokens; row t of the call belongs to the sequence s with cu[s] <= t < cu[s + 1]).  The kernels
+read all of a batch on the device, so a captured CUDA graph follows lengths and tables that change
+between replays.  Lengths or pages outside their bounds are never followed; they set
+STATUS_INDEX_RANGE in the device status word.
+
+`PagedKVCache` owns the tensors and the pages of its sequences; the functions are the operators.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from . import _lib
+
+QUANT_BLOCK = 16  # tokens that share a scale
+PAGE_SIZES = (16, 32, 64, 128, 256)
+_WIDTHS = (32, 64, 128, 256)
+
+
+def padded_head_dim(head_dim: int) -> int:
+    """Head width as stored: rounded up to 32, 64, 128 or 256."""
+    for width in _WIDTHS:
+        if 0 < head_dim <= width:
+            return width
+    raise ValueError("head_dim must be in [1, 256]")
+
+
+def _check_cache(codes: Tensor, scales: Tensor, what: str, ndim: int = 5) -> None:
+    if not codes.is_cuda:
+        raise RuntimeError(f"{what} requires CUDA; the key/value cache is GPU-only")
+    if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
+        raise TypeError(f"{what}: codes must be int8 and scales float32")
+    shape = codes.shape
+    if (codes.dim() != ndim or shape[-4] != 2
+            or scales.shape != shape[:-2] + (shape[-2] // QUANT_BLOCK,)):
+        raise ValueError(f"{what}: codes must be [..., pages, 2, heads, page_size, width] and scales "
+                         "[..., pages, 2, heads, page_size / 16]")
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f"{what}: codes and scales must be contiguous")
+
+
+def _check_batch(page_table: Tensor, lens: Tensor, cu_tokens: Tensor, what: str) -> None:
+    if not (page_table.dtype is lens.dtype is cu_tokens.dtype is torch.int32):
+        raise TypeError(f"{what}: page_table, lengths and cu_tokens must be int32")
+    seqs = lens.numel()
+    if (page_table.dim() != 2 or page_table.shape[0] != seqs or cu_tokens.numel() != seqs + 1):
+        raise ValueError(f"{what}: page_table must be [seqs, pages], lengths [seqs] and cu_tokens "
+                         "[seqs + 1]")
+    if not (page_table.is_contiguous() and lens.is_contiguous() and cu_tokens.is_contiguous()):
+        raise ValueError(f"{what}: page_table, lengths and cu_tokens must be contiguous")
+    if not (page_table.is_cuda and lens.is_cuda and cu_tokens.is_cuda):
+        raise RuntimeError(f"{what} requires CUDA; the batch is read on the device")
+
+
+def kv_append(codes: Tensor, scales: Tensor, page_table: Tensor, kv_lens: Tensor, cu_tokens: Tensor,
+              k: Tensor, v: Tensor) -> None:
+    """Quantises the newest keys and values k, v [tokens, kv_heads, head_dim] (float32 or bfloat16,
+    any token and head strides) into their pages, in place.
+
+    A block's scale is max|x| / 127 over its tokens and only grows while its tokens arrive; codes
+    already held are re-rounded when it does.  No two sequences may append into one page."""
+    _check_cache(codes, scales, "kv_append")
+    _check_batch(page_table, kv_lens, cu_tokens, "kv_append")
+    pages, _, heads, page_size, width = codes.shape
+    if k.shape != v.shape or k.dim() != 3 or k.shape[1] != heads or k.shape[2] > width:
+        raise ValueError("kv_append: k and v must be [tokens, kv_heads, head_dim] of the cache's heads")
+    if k.dtype is not v.dtype or k.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("kv_append: k and v must both be float32 or bfloat16")
+    if k.device != codes.device or v.device != codes.device:
+        raise ValueError("kv_append: k and v must be on the cache's device")
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.stride(2) != 1:
+        v = v.contiguous()
+    tokens, _, head_dim = k.shape
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    ev = _lib.prof_start(k)
+    _lib.check(_lib.lib().rt_kv_append(
+        codes.data_ptr(), scales.data_ptr(), pages, heads, page_size, width, page_table.data_ptr(),
+        page_table.shape[1], kv_lens.data_ptr(), cu_tokens.data_ptr(), kv_lens.numel(), tokens,
+        k.data_ptr(), v.data_ptr(), _lib.dtype_code(k), head_dim, kt, kh, vt, vh,
+        _lib.stream_of(codes)))
+    _lib.prof_stop(ev, "kv_append", k, 0.0, 2 * k.numel() * (k.element_size() + 1))
+
+
+def kv_read(codes: Tensor, scales: Tensor, page_table: Tensor, starts: Tensor, cu_tokens: Tensor,
+            tokens: int, head_dim: int | None = None, *, dtype: torch.dtype = torch.bfloat16
+            ) -> tuple[Tensor, Tensor]:
+    """(k, v) [tokens, kv_heads, head_dim]: the values of the cache at positions starts[s] + i of
+    each sequence, row cu_tokens[s] + i; code · scale, rounded once to dtype."""
+    _check_cache(codes, scales, "kv_read")
+    _check_batch(page_table, starts, cu_tokens, "kv_read")
+    pages, _, heads, page_size, width = codes.shape
+    head_dim = width if head_dim is None else head_dim
+    if tokens < 0 or not 0 < head_dim <= width:
+        raise ValueError("kv_read: tokens must be >= 0 and head_dim in [1, stored width]")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("kv_read: dtype must be float32 or bfloat16")
+    out = torch.empty((2, tokens, heads, head_dim), device=codes.device, dtype=dtype)
+    k, v = out[0], out[1]
+    ev = _lib.prof_start(out)
+    _lib.check(_lib.lib().rt_kv_read(
+        codes.data_ptr(), scales.data_ptr(), pages, heads, page_size, width, page_table.data_ptr(),
+        page_table.shape[1], starts.data_ptr(), cu_tokens.data_ptr(), starts.numel(), tokens, head_dim,
+        k.data_ptr(), v.data_ptr(), _lib.dtype_code(out), _lib.stream_of(codes)))
+    _lib.prof_stop(ev, "kv_read", out, 0.0, out.numel() * (out.element_size() + 1))
+    return k, v
+
+
+def kv_copy_pages(codes: Tensor, scales: Tensor, src: Tensor, dst: Tensor, *,
+                  page_table: Tensor | None = None) -> None:
+    """Copies pages src[i] to dst[i] (int32 on the device) in every layer of codes [layers, pages, ...]
+    and scales, in one launch.  page_table, when given, has every entry equal to src[i] replaced by
+    dst[i]: the pages are moved.  No page may be source and destination, or destination twice."""
+    _check_cache(codes, scales, "kv_copy_pages", ndim=6)
+    if src.dtype is not torch.int32 or dst.dtype is not torch.int32 or (
+            page_table is not None and page_table.dtype is not torch.int32):
+        raise TypeError("kv_copy_pages: src, dst and page_table must be int32")
+    if src.dim() != 1 or src.shape != dst.shape:
+        raise ValueError("kv_copy_pages: src and dst must be 1-D of one length")
+    if not (src.is_cuda and dst.is_cuda and (page_table is None or page_table.is_cuda)):
+        raise RuntimeError("kv_copy_pages requires CUDA; page lists are read on the device")
+    if not (src.is_contiguous() and dst.is_contiguous()
+            and (page_table is None or page_table.is_contiguous())):
+        raise ValueError("kv_copy_pages: src, dst and page_table must be contiguous")
+    layers, pages, _, heads, page_size, width = codes.shape
+    ev = _lib.prof_start(codes)
+    _lib.check(_lib.lib().rt_kv_copy_pages(
+        codes.data_ptr(), scales.data_ptr(), layers, pages, heads, page_size, width, src.data_ptr(),
+        dst.data_ptr(), src.numel(), _lib.ptr(page_table),
+        0 if page_table is None else page_table.numel(), _lib.stream_of(codes)))
+    _lib.prof_stop(ev, "kv_copy_pages", codes, 0.0,
+                   2 * layers * src.numel() * 2 * heads * page_size * (width + 4 / QUANT_BLOCK))
+
+
+def kv_attention(q: Tensor, codes: Tensor, scales: Tensor, page_table: Tensor, kv_lens: Tensor,
+                 cu_tokens: Tensor, *, softmax_scale: float | None = None,
+                 out: Tensor | None = None) -> Tensor:
+    """Causal attention of the newest tokens q [tokens, heads, head_dim] (float32 or bfloat16, any
+    token and head strides) over the cache, their own keys and values included (append them first).
+
+    Query head h reads key/value head h // (heads / kv_heads).  softmax_scale defaults to
+    1 / sqrt(head_dim).  A row that sees no key (or belongs to no sequence) gives zeros.  `out`, when
+    given, has q's shape and dtype and a unit innermost stride."""
+    _check_cache(codes, scales, "kv_attention")
+    _check_batch(page_table, kv_lens, cu_tokens, "kv_attention")
+    pages, _, kv_heads, page_size, width = codes.shape
+    if q.dim() != 3 or q.shape[2] > width or q.shape[1] % kv_heads != 0 or q.shape[1] == 0:
+        raise ValueError("kv_attention: q must be [tokens, heads, head_dim] with heads a multiple of "
+                         "the cache's heads")
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("kv_attention: q must be float32 or bfloat16")
+    if q.device != codes.device:
+        raise ValueError("kv_attention: q must be on the cache's device")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    tokens, heads, head_dim = q.shape
+    if out is None:
+        out = torch.empty((tokens, heads, head_dim), device=q.device, dtype=q.dtype)
+    elif (out.shape != q.shape or out.dtype is not q.dtype or out.stride(2) != 1
+          or out.device != q.device):
+        raise ValueError("kv_attention: out must have q's shape, dtype and device and a unit last stride")
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(head_dim)
+    lib = _lib.lib()
+    seqs = kv_lens.numel()
+    nbytes = lib.rt_kv_attention_workspace_bytes(seqs, tokens, heads, kv_heads, width)
+    # allocated per call: the caching allocator keeps calls on different streams apart
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    qt, qh, _ = q.stride()
+    ot, oh, _ = out.stride()
+    ev = _lib.prof_start(q)
+    _lib.check(lib.rt_kv_attention(
+        q.data_ptr(), _lib.dtype_code(q), qt, qh, heads, head_dim, codes.data_ptr(),
+        scales.data_ptr(), pages, kv_heads, page_size, width, page_table.data_ptr(),
+        page_table.shape[1], kv_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens,
+        softmax_scale, out.data_ptr(), ot, oh, _lib.ptr(ws), nbytes, _lib.stream_of(q)))
+    # the lengths are on the device: only the rows' own bytes are counted here
+    _lib.prof_stop(ev, "kv_attention", q, 0.0, 2 * q.numel() * q.element_size())
+    return out
+
+
+@dataclass(frozen=True)
+class CacheBatch:
+    """The sequences of one call, as the kernels read them (`PagedKVCache.reserve`)."""
+
+    page_table: Tensor
+    kv_lens: Tensor
+    cu_tokens: Tensor
+    positions: Tensor  # int64 [tokens]: position of each new row in its sequence
+    n_tokens: int
+
+
+class PagedKVCache:
+    """Key/value cache of all layers of a model in one pool of pages.
+
+    Sequences are integer ids.  `reserve` extends sequences by their newest tokens and returns the
+    batch that `append` and `attend` take, layer by layer.  `fork` shares pages; a shared page is
+    copied when a sequence is about to write into it.  `free` and `truncate` give pages back, and
+    `compact` moves the pages in use to the front of the pool.  The bookkeeping is on the host and
+    nothing in it waits for the device."""
+
+    def __init__(self, n_layer: int, n_kv_head: int, head_dim: int, *, n_pages: int,
+                 page_size: int = 64, device: torch.device | str = "cuda") -> None:
+        if min(n_layer, n_kv_head, n_pages) <= 0:
+            raise ValueError("n_layer, n_kv_head and n_pages must be positive")
+        if page_size not in PAGE_SIZES:
+            raise ValueError("page_size must be 16, 32, 64, 128 or 256")
+        width = padded_head_dim(head_dim)
+        self.n_layer, self.n_kv_head, self.head_dim = n_layer, n_kv_head, head_dim
+        self.n_pages, self.page_size = n_pages, page_size
+        shape = (n_layer, n_pages, 2, n_kv_head, page_size)
+        self.codes = torch.zeros((*shape, width), device=device, dtype=torch.int8)
+        self.scales = torch.zeros((*shape[:-1], page_size // QUANT_BLOCK), device=device,
+                                  dtype=torch.float32)
+        self._free = list(range(n_pages - 1, -1, -1))  # popped from the end: low pages first
+        self._refs = [0] * n_pages
+        self._pages: dict[int, list[int]] = {}
+        self._lens: dict[int, int] = {}
+        self._next = 0
+
+    # ------------------------------------------------------------------ sequences
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def new_sequence(self) -> int:
+        seq = self._next
+        self._next += 1
+        self._pages[seq] = []
+        self._lens[seq] = 0
+        return seq
+
+    def length(self, seq: int) -> int:
+        self._known(seq)
+        return self._lens[seq]
+
+    def pages(self, seq: int) -> list[int]:
+        self._known(seq)
+        return list(self._pages[seq])
+
+    def fork(self, seq: int) -> int:
+        """A new sequence with the same tokens; the pages are shared until one of the two writes."""
+        self._known(seq)
+        new = self.new_sequence()
+        self._pages[new] = list(self._pages[seq])
+        self._lens[new] = self._lens[seq]
+        for page in self._pages[new]:
+            self._refs[page] += 1
+        return new
+
+    def free(self, seq: int) -> None:
+        self._known(seq)
+        for page in self._pages.pop(seq):
+            self._release(page)
+        del self._lens[seq]
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Drops the tokens from `length` on (rejected drafts)."""
+        self._known(seq)
+        if not 0 <= length <= self._lens[seq]:
+            raise ValueError("truncate: length must be in [0, the sequence's length]")
+        keep = -(-length // self.page_size)
+        for page in self._pages[seq][keep:]:
+            self._release(page)
+        del self._pages[seq][keep:]
+        self._lens[seq] = length
+
+    def _known(self, seq: int) -> None:
+        if seq not in self._pages:
+            raise KeyError(f"unknown sequence {seq}")
+
+    def _release(self, page: int) -> None:
+        self._refs[page] -= 1
+        if self._refs[page] == 0:
+            self._free.append(page)
+
+    # ------------------------------------------------------------------ batches
+    def reserve(self, seqs: list[int], new_tokens: list[int] | int = 1) -> CacheBatch:
+        """Extends each sequence by its count of newest tokens and returns the batch for them.
+        Raises RuntimeError, with nothing changed, when the pool has too few free pages."""
+        counts = [new_tokens] * len(seqs) if isinstance(new_tokens, int) else list(new_tokens)
+        if len(counts) != len(seqs) or len(set(seqs)) != len(seqs):
+            raise ValueError("reserve: one count per sequence, and each sequence once")
+        if any(n < 0 for n in counts):
+            raise ValueError("reserve: counts must be >= 0")
+        need, refs = 0, {}
+        for seq, n in zip(seqs, counts):
+            self._known(seq)
+            need += max(0, -(-(self._lens[seq] + n) // self.page_size) - len(self._pages[seq]))
+            page = self._written_page(seq, n)
+            if page is not None:
+                left = refs.get(page, self._refs[page])
+                if left > 1:
+                    need += 1
+                    refs[page] = left - 1
+        if need > len(self._free):
+            raise RuntimeError(f"key/value cache: {need} pages needed, {len(self._free)} free")
+        src, dst = [], []
+        for seq, n in zip(seqs, counts):
+            page = self._written_page(seq, n)
+            if page is not None and self._refs[page] > 1:
+                own = self._take()
+                self._refs[page] -= 1
+                self._pages[seq][self._lens[seq] // self.page_size] = own
+                src.append(page)
+                dst.append(own)
+            self._lens[seq] += n
+            pages = self._pages[seq]
+            while len(pages) * self.page_size < self._lens[seq]:
+                pages.append(self._take())
+        if src:
+            self._copy(src, dst)
+        return self._batch(seqs, counts)
+
+    def _written_page(self, seq: int, n: int) -> int | None:
+        """The partly filled page that the next n tokens of the sequence begin in, if any."""
+        length = self._lens[seq]
+        return self._pages[seq][length // self.page_size] if n and length % self.page_size else None
+
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._refs[page] = 1
+        return page
+
+    def _ints(self, values: list[int]) -> Tensor:
+        t = torch.tensor(values, dtype=torch.int32)
+        if self.codes.is_cuda:
+            return t.pin_memory().to(self.codes.device, non_blocking=True)
+        return t
+
+    def _batch(self, seqs: list[int], counts: list[int]) -> CacheBatch:
+        # one host-to-device copy holds the table, the lengths, the prefix sums and the positions
+        width = max([len(self._pages[s]) for s in seqs], default=0)
+        rows = [p for s in seqs for p in self._pages[s] + [0] * (width - len(self._pages[s]))]
+        cu = [0]
+        for n in counts:
+            cu.append(cu[-1] + n)
+        positions = [p for s, n in zip(seqs, counts) for p in range(self._lens[s] - n, self._lens[s])]
+        packed = self._ints(rows + [self._lens[s] for s in seqs] + cu + positions)
+        a = len(rows)
+        b = a + len(seqs)
+        c = b + len(cu)
+        return CacheBatch(packed[:a].view(len(seqs), width), packed[a:b], packed[b:c],
+                          packed[c:].long(), cu[-1])
+
+    # ------------------------------------------------------------------ operators
+    def append(self, layer: int, batch: CacheBatch, k: Tensor, v: Tensor) -> None:
+        if k.shape[0] != batch.n_tokens or k.shape[-1] != self.head_dim:
+            raise ValueError("append: k must hold the batch's tokens and the cache's head width")
+        kv_append(self.codes[layer], self.scales[layer], batch.page_table, batch.kv_lens,
+                  batch.cu_tokens, k, v)
+
+    def attend(self, layer: int, batch: CacheBatch, q: Tensor, *,
+               softmax_scale: float | None = None) -> Tensor:
+        if q.shape[0] != batch.n_tokens or q.shape[-1] != self.head_dim:
+            raise ValueError("attend: q must hold the batch's tokens and the cache's head width")
+        return kv_attention(q, self.codes[layer], self.scales[layer], batch.page_table, batch.kv_lens,
+                            batch.cu_tokens, softmax_scale=softmax_scale)
+
+    def read(self, layer: int, seq: int, start: int = 0, end: int | None = None, *,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
+        """(k, v) [end - start, kv_heads, head_dim] of one sequence."""
+        self._known(seq)
+        end = self._lens[seq] if end is None else end
+        if not 0 <= start <= end <= self._lens[seq]:
+            raise ValueError("read: 0 <= start <= end <= the sequence's length")
+        pages = self._pages[seq]
+        packed = self._ints(pages + [start, 0, end - start])
+        n = len(pages)
+        return kv_read(self.codes[layer], self.scales[layer], packed[:n].view(1, n),
+                       packed[n:n + 1], packed[n + 1:], end - start, self.head_dim, dtype=dtype)
+
+    def _copy(self, src: list[int], dst: list[int]) -> None:
+        both = self._ints(src + dst)
+        kv_copy_pages(self.codes, self.scales, both[:len(src)], both[len(src):])
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool (one launch over all layers) and returns
+        how many were moved.  Batches reserved before hold the old pages: reserve again."""
+        used = sorted((p for p in range(self.n_pages) if self._refs[p]), reverse=True)
+        live = len(used)
+        holes = [p for p in range(live) if not self._refs[p]]
+        src = used[:len(holes)]  # the highest pages; every one of them lies behind every hole
+        if not src:
+            return 0
+        moved = dict(zip(src, holes))
+        self._copy(src, holes)
+        for old, new in moved.items():
+            self._refs[new], self._refs[old] = self._refs[old], 0
+        for seq, pages in self._pages.items():
+            self._pages[seq] = [moved.get(p, p) for p in pages]
+        self._free = list(range(self.n_pages - 1, live - 1, -1))
+        return len(src)

@@ -1,0 +1,604 @@
+"""GPU: the paged int8 key/value cache operators against plain implementations in 64 bits.
+
+Bars, from the arithmetic:
+* append: the scale is one fp32 division (relative error 2^-24) and a code one more division and a
+  rounding: |code - x / s| <= 1/2 + 127·2^-22 with s the stored scale; held codes likewise.
+* read: one fp32 product, equal to torch's; bf16 its rounding.
+* attention, fp32: with n keys, width D, X = max sum_d |c q_d k_d| and M = max |v|, a score is off by at
+  most (D + 8)·2^-24·X, a weight by twice that, a sum by n·2^-24:
+  |o - ref| <= (2 (D + 8) X + 2 n + 16)·2^-24·M.  bf16 adds a weight rounded to bf16 (2^-8·M at most,
+  as its numerator only) and the output's rounding (2^-8·M).  In the 2-norm rounding errors average:
+  scores are off by about sqrt(D)·2^-24·X and weights by twice that, the sums and exponentials by
+  less than 1e-5: the bar is 1e-5 + 2 sqrt(D)·2^-24·X; the two bf16 roundings add
+  2^-8/sqrt(12)·sqrt(2) = 1.6e-3 of the output, for which the bar has 4e-3 more.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from local_ai_training_b200 import _lib, kv_cache
+from local_ai_training_b200.kv_cache import QUANT_BLOCK, PagedKVCache, padded_head_dim
+
+pytestmark = pytest.mark.gpu
+
+TINY = torch.finfo(torch.float32).tiny
+
+
+class _Case:
+    """A cache filled with random codes, a batch over shuffled pages, and its values in 64 bits."""
+
+    def __init__(self, dev, lens, news, *, heads=4, kv_heads=2, dim=64, page=32, seed=0, extra_rows=0):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        self.dev, self.lens, self.news = dev, lens, news
+        self.heads, self.kv_heads, self.dim, self.page = heads, kv_heads, dim, page
+        width = padded_head_dim(dim)
+        need = [-(-n // page) for n in lens]
+        pages = sum(need) + 2
+        self.codes = torch.randint(-127, 128, (pages, 2, kv_heads, page, width), device=dev, generator=g,
+                                   dtype=torch.int8)
+        self.codes[..., dim:] = 0
+        self.scales = torch.rand(pages, 2, kv_heads, page // QUANT_BLOCK, device=dev, generator=g) * 0.02 + 1e-3
+        order = torch.randperm(pages, device=dev, generator=g).to(torch.int32)
+        table = torch.full((len(lens), max(need + [1])), -1, device=dev, dtype=torch.int32)
+        at = 0
+        for s, n in enumerate(need):
+            table[s, :n] = order[at:at + n]
+            at += n
+        self.table = table
+        self.kv_lens = torch.tensor(lens, device=dev, dtype=torch.int32)
+        cu = [0]
+        for n in news:
+            cu.append(cu[-1] + n)
+        self.cu = torch.tensor(cu, device=dev, dtype=torch.int32)
+        self.tokens = cu[-1] + extra_rows
+        self.gen = g
+
+    def values(self, s):
+        """[2, kv_heads, len, dim] in 64 bits."""
+        n = -(-self.lens[s] // self.page)
+        p = self.table[s, :n].long()
+        x = self.codes[p].double() * self.scales[p].double().repeat_interleave(QUANT_BLOCK, -1)[..., None]
+        x = x.permute(1, 2, 0, 3, 4).reshape(2, self.kv_heads, -1, self.codes.shape[-1])
+        return x[:, :, :self.lens[s], :self.dim]
+
+    def attention(self, q, scale=None):
+        """Reference output in 64 bits, the largest |v|, the largest sum |c q k|."""
+        c = 1 / math.sqrt(self.dim) if scale is None else scale
+        out = torch.zeros(q.shape, device=self.dev, dtype=torch.float64)
+        big_v, big_x, at, group = 0.0, 0.0, 0, self.heads // self.kv_heads
+        for s, (length, n) in enumerate(zip(self.lens, self.news)):
+            if n and length:
+                k, v = self.values(s).repeat_interleave(group, 1)
+                x = q[at:at + n].double().transpose(0, 1)
+                t = c * x @ k.transpose(1, 2)
+                seen = torch.arange(length, device=self.dev) <= (
+                    torch.arange(n, device=self.dev) + length - n)[:, None]
+                w = torch.softmax(t.masked_fill(~seen, -math.inf), -1)
+                w = torch.where(seen.any(-1)[:, None], w, 0.0)  # a row that sees no key
+                out[at:at + n] = (w @ v).transpose(0, 1)
+                big_v = max(big_v, v.abs().max().item())
+                big_x = max(big_x, (abs(c) * x.abs() @ k.abs().transpose(1, 2)).max().item())
+            at += n
+        return out, big_v, big_x
+
+    def queries(self, dtype):
+        q = torch.randn(self.tokens, self.heads, self.dim, device=self.dev, generator=self.gen)
+        return (q * 1.5).to(dtype)
+
+    def check(self, got, q, scale=None):
+        ref, big_v, big_x = self.attention(q, scale)
+        err = (got.double() - ref).abs().max().item() if got.numel() else 0.0
+        bound = (2 * (self.dim + 8) * big_x + 2 * max(self.lens + [0]) + 16) * 2.0 ** -24 * big_v
+        rel = 1e-5 + 2 * math.sqrt(self.dim) * 2.0 ** -24 * big_x
+        if q.dtype == torch.bfloat16:
+            bound += 2 * 2.0 ** -8 * big_v
+            rel += 4e-3
+        assert err <= bound, (err, bound)
+        if ref.norm() > 0:
+            assert (got.double() - ref).norm() <= rel * ref.norm()
+
+    def run(self, q, **kw):
+        return kv_cache.kv_attention(q, self.codes, self.scales, self.table, self.kv_lens, self.cu, **kw)
+
+
+def _status(dev):
+    return _lib.device_status(dev, clear=True)
+
+
+# ------------------------------------------------------------------------------------ attention
+LENS = [
+    ([1], [1]),
+    ([16], [1]),
+    ([17, 15, 1, 33], [1, 1, 1, 1]),
+    ([1000, 3, 64, 65, 63], [1, 3, 2, 65, 1]),
+    ([40, 0, 129], [7, 0, 0]),           # a sequence with nothing, one with no newest tokens
+    ([300, 77], [130, 77]),              # prompt pieces, one from its beginning
+    ([257], [257]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens,news", LENS, ids=[f"{l}+{n}".replace(" ", "") for l, n in LENS])
+def test_attention_lengths(cuda_device, lens, news, dtype):
+    case = _Case(cuda_device, lens, news)
+    q = case.queries(dtype)
+    case.check(case.run(q), q)
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 16, 32, 40, 64, 80, 128, 200, 256])
+def test_attention_head_widths(cuda_device, dim, dtype):
+    for news in ([1, 1, 1], [40, 2, 131]):
+        case = _Case(cuda_device, [150, 18, 200], news, dim=dim, seed=dim)
+        q = case.queries(dtype)
+        case.check(case.run(q), q)
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 3), (8, 1), (12, 4), (7, 1), (32, 8), (48, 2), (16, 16),
+                                            (40, 1)])
+def test_attention_shared_heads(cuda_device, heads, kv_heads, dtype):
+    for lens, news in (([90, 130, 5], [1, 1, 1]), ([90, 130, 5], [3, 1, 2]), ([700, 400], [300, 20])):
+        case = _Case(cuda_device, lens, news, heads=heads, kv_heads=kv_heads, dim=128, seed=heads)
+        q = case.queries(dtype)
+        case.check(case.run(q), q)
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("page", kv_cache.PAGE_SIZES)
+def test_attention_page_sizes_and_long_splits(cuda_device, page):
+    for lens, news in (([5000, 1, 777], [1, 1, 1]), ([3001], [200]), ([40000], [1])):
+        case = _Case(cuda_device, lens, news, heads=8, kv_heads=4, dim=128, page=page, seed=page)
+        for dtype in (torch.bfloat16, torch.float32):
+            q = case.queries(dtype)
+            case.check(case.run(q), q)
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_many_sequences(cuda_device, dtype):
+    lens = [(37 * i) % 211 for i in range(300)]
+    news = [0 if n == 0 else (i % 4 if i % 7 else min(n, 40)) for i, n in enumerate(lens)]
+    news = [min(a, b) for a, b in zip(news, lens)]
+    case = _Case(cuda_device, lens, news, heads=8, kv_heads=2, dim=64, page=16)
+    q = case.queries(dtype)
+    case.check(case.run(q), q)
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("news", [[1, 1, 1], [60, 1, 100]])
+def test_attention_strides_and_out(cuda_device, dtype, news):
+    """q as a part of a q|k|v row, heads before tokens, unaligned rows, and a strided out."""
+    case = _Case(cuda_device, [100, 20, 300], news, heads=4, kv_heads=4, dim=64)
+    q = case.queries(dtype)
+    t, h, d = q.shape
+    qkv = torch.full((t, 3, h, d), float("nan"), device=cuda_device, dtype=dtype)
+    qkv[:, 1] = q
+    by_head = q.transpose(0, 1).contiguous().transpose(0, 1)
+    odd = torch.empty(t * h * d + 1, device=cuda_device, dtype=dtype)[1:].view(t, h, d)
+    odd.copy_(q)
+    wide = torch.empty(t, h, d + 3, device=cuda_device, dtype=dtype)[..., :d]
+    wide.copy_(q)
+    inner = q.transpose(1, 2).contiguous().transpose(1, 2)
+    first = case.run(q)
+    case.check(first, q)
+    for view in (qkv[:, 1], by_head, odd, wide, inner):
+        assert torch.equal(case.run(view), first)
+    room = torch.full((t, h, 2 * d), 7.0, device=cuda_device, dtype=dtype)
+    out = room[..., d // 2:d // 2 + d]
+    assert case.run(q, out=out) is out
+    assert torch.equal(out, first)
+    assert (room[..., :d // 2] == 7).all() and (room[..., d // 2 + d:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("news", [[2, 1], [90, 1]])
+def test_attention_reads_nothing_past_the_length(cuda_device, dtype, news):
+    """Stale codes behind the length and NaN scales of unused blocks leave no trace."""
+    case = _Case(cuda_device, [97, 40], news, heads=4, kv_heads=2, dim=128, page=64)
+    q = case.queries(dtype)
+    first = case.run(q)
+    case.check(first, q)
+    for s, n in enumerate(case.lens):
+        page = case.table[s, n // 64].long()
+        case.codes[page, :, :, n % 64:] = 127
+        used = -(-(n % 64) // QUANT_BLOCK)
+        case.scales[page, :, :, used:] = float("nan")
+    unused = torch.ones(case.codes.shape[0], dtype=torch.bool, device=cuda_device)
+    unused[case.table[case.table >= 0].long()] = False
+    case.scales[unused] = float("inf")
+    assert torch.equal(case.run(q), first)
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_rows_without_keys_are_zero(cuda_device, dtype):
+    """More newest tokens than keys (the first ones see none), rows of no sequence, an empty batch."""
+    for dim, news in ((64, [5, 2]), (128, [140, 2])):
+        case = _Case(cuda_device, [3, 20], news, dim=dim, extra_rows=6)
+        q = case.queries(dtype)
+        out = torch.full_like(q, float("nan"))
+        case.run(q, out=out)
+        case.check(out, q)
+        assert (out[:news[0] - 3] == 0).all() and (out[-6:] == 0).all()
+        assert _status(cuda_device) == _lib.STATUS_INDEX_RANGE  # fewer keys than newest tokens
+    empty = case.run(q[:0])
+    assert empty.shape == (0, case.heads, case.dim)
+    _status(cuda_device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+def test_attention_softmax_scale(cuda_device, dtype, scale):
+    """Uniform weights, a negative scale, and scores of hundreds (one key takes all)."""
+    for news in ([1, 3], [150, 3]):
+        case = _Case(cuda_device, [400, 50], news)
+        q = case.queries(dtype)
+        case.check(case.run(q, softmax_scale=scale), q, scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("news", [[1, 2], [70, 2]])
+def test_attention_zero_and_tiny_blocks(cuda_device, dtype, news):
+    """Blocks of zeros (the smallest scale) next to ordinary ones, and values of very different size."""
+    case = _Case(cuda_device, [200, 90], news)
+    case.codes[::2, 1] = 0
+    case.scales[::2, 1] = TINY
+    case.scales[1::2, 1, :, 0] *= 1e4
+    case.codes[::3, 0] = 0
+    case.scales[::3, 0] = TINY
+    q = case.queries(dtype)
+    case.check(case.run(q), q)
+
+
+def test_attention_bad_pages_and_lengths_are_flagged(cuda_device):
+    case = _Case(cuda_device, [60, 60], [1, 1])
+    q = case.queries(torch.bfloat16)
+    first = case.run(q)
+    table = case.table
+    case.table = table.clone()
+    case.table[1, 0] = 10 ** 6  # no such page: its keys do not exist
+    out = case.run(q)
+    assert _status(cuda_device) == _lib.STATUS_INDEX_RANGE
+    assert torch.equal(out[0], first[0]) and torch.isfinite(out).all()
+    case.table = table
+    case.kv_lens = torch.tensor([60, 10 ** 6], device=cuda_device, dtype=torch.int32)
+    case.table = torch.where(table < 0, 0, table).contiguous()
+    out = case.run(q)  # cut to the table's room
+    assert _status(cuda_device) == _lib.STATUS_INDEX_RANGE
+    assert torch.equal(out[0], first[0]) and torch.isfinite(out).all()
+
+
+def test_attention_is_repeatable_and_follows_a_replayed_graph(cuda_device):
+    case = _Case(cuda_device, [3000, 500], [1, 1], heads=8, kv_heads=8, dim=128)
+    q = case.queries(torch.bfloat16)
+    first = case.run(q)
+    for _ in range(3):
+        assert torch.equal(case.run(q), first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = case.run(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            replayed = case.run(q)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, first)
+    graph.replay()
+    assert torch.equal(replayed, first)
+    case.lens = [1234, 1]
+    case.kv_lens.copy_(torch.tensor(case.lens, dtype=torch.int32))
+    graph.replay()
+    case.check(replayed, q)
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_attention_pool_over_32_bits(cuda_device, new):
+    """Pages behind 2^32 bytes of codes."""
+    pages, heads, page, dim = 17000, 16, 64, 128  # 4.46e9 bytes
+    codes = torch.zeros(pages, 2, heads, page, dim, device=cuda_device, dtype=torch.int8)
+    scales = torch.full((pages, 2, heads, page // QUANT_BLOCK), 0.01, device=cuda_device)
+    small = _Case(cuda_device, [260], [new], heads=heads, kv_heads=heads, dim=dim, page=page)
+    far = torch.tensor([16999, 16400, 3, 16996, 16990], device=cuda_device)
+    near = small.table[0, :5].long()
+    codes[far], scales[far] = small.codes[near], small.scales[near]
+    q = small.queries(torch.bfloat16)
+    table = far.to(torch.int32)[None].contiguous()
+    got = kv_cache.kv_attention(q, codes, scales, table, small.kv_lens, small.cu)
+    assert torch.equal(got, small.run(q))
+    x = torch.randn(new, heads, dim, device=cuda_device)
+    kv_cache.kv_append(codes, scales, table, small.kv_lens, small.cu, x, -x)
+    kv_cache.kv_append(small.codes, small.scales, small.table, small.kv_lens, small.cu, x, -x)
+    assert torch.equal(codes[far], small.codes[near]) and torch.equal(scales[far], small.scales[near])
+    src, dst = far[:1].to(torch.int32), torch.tensor([16800], device=cuda_device, dtype=torch.int32)
+    kv_cache.kv_copy_pages(codes[None], scales[None], src, dst)
+    assert torch.equal(codes[16800], codes[16999])
+
+
+def test_attention_refusals(cuda_device):
+    case = _Case(cuda_device, [20], [1])
+    q = case.queries(torch.bfloat16)
+    args = (case.codes, case.scales, case.table, case.kv_lens, case.cu)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        kv_cache.kv_attention(q.half(), *args)
+    with pytest.raises(ValueError, match="multiple of"):
+        kv_cache.kv_attention(q[:, :3], *args)
+    with pytest.raises(ValueError, match="head_dim"):
+        kv_cache.kv_attention(torch.zeros(1, 4, 65, device=cuda_device), *args)
+    with pytest.raises(TypeError, match="int8"):
+        kv_cache.kv_attention(q, case.codes.float(), *args[1:])
+    with pytest.raises(ValueError, match="scales"):
+        kv_cache.kv_attention(q, case.codes, case.scales[:1], *args[2:])
+    with pytest.raises(ValueError, match="contiguous"):
+        kv_cache.kv_attention(q, case.codes.transpose(2, 3).contiguous().transpose(2, 3), *args[1:])
+    with pytest.raises(TypeError, match="int32"):
+        kv_cache.kv_attention(q, *args[:2], case.table.long(), *args[3:])
+    with pytest.raises(ValueError, match="cu_tokens"):
+        kv_cache.kv_attention(q, *args[:4], case.cu[:1])
+    with pytest.raises(RuntimeError, match="requires CUDA"):
+        kv_cache.kv_attention(q, *args[:3], case.kv_lens.cpu(), case.cu)
+    with pytest.raises(ValueError, match="device"):
+        kv_cache.kv_attention(q.cpu(), *args)
+    with pytest.raises(ValueError, match="out must"):
+        kv_cache.kv_attention(q, *args, out=torch.empty_like(q).float())
+    with pytest.raises(ValueError, match="finite"):
+        kv_cache.kv_attention(q, *args, softmax_scale=float("nan"))
+
+
+# --------------------------------------------------------------------------------------- append
+def _append_and_check(case, k, v):
+    before, scales_before = case.codes.clone(), case.scales.double().clone()
+    kv_cache.kv_append(case.codes, case.scales, case.table, case.kv_lens, case.cu, k, v)
+    slack = 0.5 + 127 * 2.0 ** -22
+    touched = torch.zeros_like(before, dtype=torch.bool)
+    touched_scale = torch.zeros_like(scales_before, dtype=torch.bool)
+    at = 0
+    for s, (length, n) in enumerate(zip(case.lens, case.news)):
+        pos = length - n
+        while pos < length:
+            end = min(length, pos // QUANT_BLOCK * QUANT_BLOCK + QUANT_BLOCK)
+            page, row, blk = case.table[s, pos // case.page].item(), pos % case.page, pos % case.page // 16
+            x = torch.stack((k[at:at + end - pos], v[at:at + end - pos])).double().transpose(1, 2)
+            held = pos % QUANT_BLOCK
+            old = scales_before[page, :, :, blk] if held else torch.zeros_like(scales_before[page, :, :, blk])
+            want = torch.maximum(torch.maximum(x.abs().amax((-1, -2)) / 127, old),
+                                 torch.full_like(old, TINY))
+            got = case.scales[page, :, :, blk].double()
+            assert ((got - want).abs() <= 2.0 ** -23 * want).all()
+            code = case.codes[page, :, :, row:row + end - pos, :case.dim].double()
+            exact = (x / got[..., None, None]).clamp(-127, 127)
+            assert ((code - exact).abs() <= slack).all()
+            assert (case.codes[page, :, :, row:row + end - pos, case.dim:] == 0).all()
+            if held:
+                was = before[page, :, :, row - held:row].double()
+                now = case.codes[page, :, :, row - held:row].double()
+                assert ((now - was * (old / got)[..., None, None]).abs() <= slack).all()
+                same = (got == old)[..., None, None].expand_as(was)
+                assert torch.equal(now[same], was[same])
+            touched[page, :, :, row - held:row + end - pos] = True
+            touched_scale[page, :, :, blk] = True
+            at += end - pos
+            pos = end
+    assert torch.equal(case.codes[~touched], before[~touched])
+    assert torch.equal(case.scales.double()[~touched_scale], scales_before[~touched_scale])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("dim", [1, 24, 64, 100, 128, 256])
+def test_append(cuda_device, dim, page, dtype):
+    case = _Case(cuda_device, [1, 16, 17, 300, 33, 0, 50, 64], [1, 16, 1, 123, 2, 0, 33, 0], kv_heads=3,
+                 heads=3, dim=dim, page=page, seed=dim, extra_rows=4)
+    # values whose size changes from token to token, so that some block scales grow and some do not
+    x = torch.randn(case.tokens, 2, 3, dim, device=cuda_device, generator=case.gen)
+    x *= torch.rand(case.tokens, 1, 3, 1, device=cuda_device, generator=case.gen) * 3
+    _append_and_check(case, x[:, 0].to(dtype), x[:, 1].to(dtype))
+    assert _status(cuda_device) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_append_strides(cuda_device, dtype):
+    """k and v as parts of q|k|v rows, heads before tokens, unaligned rows, a strided innermost."""
+    make = lambda: _Case(cuda_device, [70, 33], [40, 1], kv_heads=4, heads=4, dim=64)  # noqa: E731
+    first = make()
+    x = torch.randn(first.tokens, 3, 4, 64, device=cuda_device).to(dtype)
+    k, v = x[:, 1], x[:, 2]
+    _append_and_check(first, k, v)
+    t = first.tokens
+    odd = torch.empty(t * 256 + 1, device=cuda_device, dtype=dtype)[1:].view(t, 4, 64)
+    odd.copy_(k)
+    by_head = v.transpose(0, 1).contiguous().transpose(0, 1)
+    inner = v.transpose(1, 2).contiguous().transpose(1, 2)
+    for kk, vv in ((k.contiguous(), by_head), (odd, v), (k, inner)):
+        case = make()
+        kv_cache.kv_append(case.codes, case.scales, case.table, case.kv_lens, case.cu, kk, vv)
+        assert torch.equal(case.codes, first.codes) and torch.equal(case.scales, first.scales)
+
+
+def test_append_token_by_token_keeps_values_within_the_growth_of_the_scale(cuda_device):
+    """One token at a time: each growth re-rounds a held code once, half a step of the new scale.
+    16 tokens grow a scale at most 15 times, so a value is off by at most 16 half steps of the last."""
+    cache = PagedKVCache(1, 2, 64, n_pages=4, page_size=16, device=cuda_device)
+    seq = cache.new_sequence()
+    torch.manual_seed(5)
+    x = torch.randn(40, 2, 64, device=cuda_device) * torch.linspace(0.1, 2, 40, device=cuda_device)[:, None, None]
+    for i in range(40):
+        batch = cache.reserve([seq])
+        cache.append(0, batch, x[i:i + 1], -x[i:i + 1])
+    k, v = cache.read(0, seq, dtype=torch.float32)
+    assert torch.equal(k, -v)
+    for at in range(0, 40, 16):
+        part = x[at:at + 16]
+        step = part.abs().amax((0, 2), keepdim=True) / 127
+        err = (k[at:at + 16] - part).abs()
+        assert (err <= 8.01 * step).all()
+        assert (err[-1] <= 0.501 * step[0]).all()  # the newest token was rounded once
+
+
+def test_append_odd_values_are_stored_and_flagged(cuda_device):
+    case = _Case(cuda_device, [16, 16], [16, 16])
+    x = torch.randn(32, 2, 64, device=cuda_device)
+    clean = x.clone()
+    x[3, 0, 5], x[4, 1, 6], x[5, 0, 7] = float("nan"), float("inf"), -float("inf")
+    kv_cache.kv_append(case.codes, case.scales, case.table, case.kv_lens, case.cu, x, clean)
+    assert _status(cuda_device) == _lib.STATUS_NONFINITE_KV
+    page = case.table[0, 0].long()
+    assert case.codes[page, 0, 0, 3, 5] == 0 and case.codes[page, 0, 1, 4, 6] == 127
+    assert case.codes[page, 0, 0, 5, 7] == -127 and torch.isfinite(case.scales).all()
+    case = _Case(cuda_device, [16], [16])
+    zero = torch.zeros(16, 2, 64, device=cuda_device)
+    tiny = torch.full_like(zero, 1e-40)
+    kv_cache.kv_append(case.codes, case.scales, case.table, case.kv_lens, case.cu, zero, tiny)
+    page = case.table[0, 0].long()
+    assert (case.scales[page, :, :, 0] == TINY).all() and (case.codes[page, :, :, :16] == 0).all()
+    assert _status(cuda_device) == 0
+
+
+def test_append_bad_pages_are_skipped_and_flagged(cuda_device):
+    case = _Case(cuda_device, [40, 40], [40, 40])
+    x = torch.randn(80, 2, 64, device=cuda_device)
+    case.table[1, 0] = -5
+    before = case.codes.clone()
+    kv_cache.kv_append(case.codes, case.scales, case.table, case.kv_lens, case.cu, x, x)
+    assert _status(cuda_device) == _lib.STATUS_INDEX_RANGE
+    changed = (case.codes != before).flatten(1).any(1).nonzero().flatten().tolist()
+    assert sorted(changed) == sorted(case.table[0].tolist() + case.table[1, 1:].tolist())
+
+
+def test_append_refusals(cuda_device):
+    case = _Case(cuda_device, [20], [1])
+    x = torch.zeros(1, 2, 64, device=cuda_device)
+    args = (case.codes, case.scales, case.table, case.kv_lens, case.cu)
+    with pytest.raises(ValueError, match="cache's heads"):
+        kv_cache.kv_append(*args, x[:, :1], x[:, :1])
+    with pytest.raises(ValueError, match="cache's heads"):
+        kv_cache.kv_append(*args, x, x[..., :32])
+    with pytest.raises(TypeError, match="both"):
+        kv_cache.kv_append(*args, x, x.bfloat16())
+    with pytest.raises(TypeError, match="both"):
+        kv_cache.kv_append(*args, x.half(), x.half())
+    with pytest.raises(ValueError, match="device"):
+        kv_cache.kv_append(*args, x.cpu(), x.cpu())
+
+
+# --------------------------------------------------------------------------------- read and copy
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 20, 64, 128, 256])
+def test_read(cuda_device, dim, dtype):
+    case = _Case(cuda_device, [100, 0, 33], [60, 0, 1], dim=dim, kv_heads=3, heads=3, extra_rows=3)
+    starts = case.kv_lens - (case.cu[1:] - case.cu[:-1])
+    k, v = kv_cache.kv_read(case.codes, case.scales, case.table, starts, case.cu, case.tokens, dim, dtype=dtype)
+    at = 0
+    for s, (length, n) in enumerate(zip(case.lens, case.news)):
+        want = case.values(s)[:, :, length - n:].transpose(1, 2)
+        # 8-bit code times 24-bit scale: exact in 64 bits, so .float() is the one rounding
+        assert torch.equal(k[at:at + n], want[0].float().to(dtype))
+        assert torch.equal(v[at:at + n], want[1].float().to(dtype))
+        at += n
+    assert (k[at:] == 0).all() and (v[at:] == 0).all()
+    assert _status(cuda_device) == 0
+
+
+def test_read_out_of_range_is_zero_and_flagged(cuda_device):
+    case = _Case(cuda_device, [64], [4])
+    starts = torch.tensor([62], device=cuda_device, dtype=torch.int32)
+    k, _ = kv_cache.kv_read(case.codes, case.scales, case.table, starts, case.cu, 4)
+    assert (k[2:] == 0).all() and (k[:2] != 0).any()
+    assert _status(cuda_device) == _lib.STATUS_INDEX_RANGE
+    with pytest.raises(ValueError, match="tokens"):
+        kv_cache.kv_read(case.codes, case.scales, case.table, starts, case.cu, -1)
+    with pytest.raises(TypeError, match="dtype"):
+        kv_cache.kv_read(case.codes, case.scales, case.table, starts, case.cu, 1, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("layers,heads,page,width,pages,n", [
+    (1, 1, 16, 32, 4, 1), (3, 2, 16, 64, 40, 17), (8, 8, 64, 64, 20, 8), (2, 3, 256, 256, 9, 3),
+    (1, 1, 16, 32, 3000, 1400)])
+def test_copy_and_move_pages(cuda_device, layers, heads, page, width, pages, n):
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    codes = torch.randint(-127, 128, (layers, pages, 2, heads, page, width), device=cuda_device,
+                          generator=g, dtype=torch.int8)
+    scales = torch.rand(layers, pages, 2, heads, page // 16, device=cuda_device, generator=g)
+    order = torch.randperm(pages, device=cuda_device, generator=g).to(torch.int32)
+    src, dst = order[:n].clone(), order[n:2 * n].clone()
+    table = torch.randint(-1, pages, (33, 41), device=cuda_device, generator=g).to(torch.int32)
+    want, want_scales = codes.clone(), scales.clone()
+    want[:, dst.long()], want_scales[:, dst.long()] = codes[:, src.long()], scales[:, src.long()]
+    moved = torch.arange(-1, pages, device=cuda_device, dtype=torch.int32)
+    moved[src.long() + 1] = dst
+    want_table = moved[table.long() + 1]
+    kv_cache.kv_copy_pages(codes, scales, src, dst, page_table=table)
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
+    assert torch.equal(table, want_table)
+    # one source for several destinations (forks), the table left alone
+    src = order[:1].expand(n).contiguous()
+    kv_cache.kv_copy_pages(codes, scales, src, dst)
+    assert (codes[:, dst.long()] == codes[:, src.long()]).all() and torch.equal(table, want_table)
+    kv_cache.kv_copy_pages(codes, scales, src[:0], dst[:0], page_table=table)
+    assert _status(cuda_device) == 0
+
+
+def test_copy_pages_bad_pages_and_refusals(cuda_device):
+    codes = torch.ones(2, 4, 2, 1, 16, 32, device=cuda_device, dtype=torch.int8)
+    scales = torch.ones(2, 4, 2, 1, 1, device=cuda_device)
+    i32 = lambda *v: torch.tensor(v, device=cuda_device, dtype=torch.int32)  # noqa: E731
+    kv_cache.kv_copy_pages(codes, scales, i32(-1, 4), i32(0, 1))
+    assert (codes == 1).all() and _status(cuda_device) == _lib.STATUS_INDEX_RANGE
+    with pytest.raises(TypeError, match="int32"):
+        kv_cache.kv_copy_pages(codes, scales, i32(0).long(), i32(1))
+    with pytest.raises(ValueError, match="one length"):
+        kv_cache.kv_copy_pages(codes, scales, i32(0, 1), i32(1))
+    with pytest.raises(RuntimeError, match="requires CUDA"):
+        kv_cache.kv_copy_pages(codes, scales, i32(0).cpu(), i32(1))
+    with pytest.raises(ValueError, match="codes must be"):
+        kv_cache.kv_copy_pages(codes[0], scales[0], i32(0), i32(1))
+
+
+# ------------------------------------------------------------------------------------- together
+def test_forks_compaction_and_drafts_read_what_they_wrote(cuda_device):
+    """Two sequences from one fork write on, a draft is cut back and written again, pages move: every
+    sequence reads its own tokens, and attention over it equals attention over a cache written once."""
+    torch.manual_seed(2)
+    cache = PagedKVCache(2, 2, 64, n_pages=24, page_size=16, device=cuda_device)
+    gone, a = cache.new_sequence(), cache.new_sequence()
+    x = torch.randn(60, 2, 64, device=cuda_device)
+
+    def write(seq, part):
+        batch = cache.reserve([seq], part.shape[0])
+        for layer in range(2):
+            cache.append(layer, batch, part * (layer + 1), -part)
+
+    write(gone, x[:40])
+    write(a, x[:20])
+    b = cache.fork(a)
+    write(a, x[20:30])
+    write(b, x[40:60])
+    cache.truncate(b, 32)
+    write(b, x[:5])
+    cache.free(gone)
+    assert cache.compact() > 0
+    for seq, want in ((a, x[:30]), (b, torch.cat((x[:20], x[40:52], x[:5])))):
+        assert cache.length(seq) == want.shape[0]
+        for layer in range(2):
+            k, v = cache.read(layer, seq, dtype=torch.float32)
+            # at most three roundings of half a step each (two growths), one step = max / 127
+            step = want.abs().max() / 127
+            assert (k / (layer + 1) - want).abs().max() <= 1.51 * step
+            assert (v + want).abs().max() <= 1.51 * step
+    batch = cache.reserve([a, b], [0, 1])
+    y = torch.randn(1, 2, 64, device=cuda_device)
+    cache.append(0, batch, y, y)
+    q = torch.randn(1, 4, 64, device=cuda_device)
+    got = cache.attend(0, batch, q)
+    k, v = cache.read(0, b, dtype=torch.float32)
+    s = torch.einsum("hgd,lhd->hgl", q[0].view(2, 2, 64).double(), k.double()) / 8
+    ref = torch.einsum("hgl,lhd->hgd", torch.softmax(s, -1), v.double()).reshape(1, 4, 64)
+    assert (got.double() - ref).norm() <= 2e-5 * ref.norm()
+    assert _status(cuda_device) == 0

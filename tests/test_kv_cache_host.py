@@ -1,0 +1,189 @@
+"""CPU: the page bookkeeping of PagedKVCache (forks, copy on write, truncation, compaction, refusals)
+and the operators' refusals.  The page copies a launch would make are recorded and carried out on
+plain lists, so the tokens every sequence would read are checked without a GPU."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from local_ai_training_b200 import kv_cache
+from local_ai_training_b200.kv_cache import PagedKVCache, padded_head_dim
+
+
+class _ListCache(PagedKVCache):
+    """Pages as lists of tokens: `write` stands for append, `_copy` for the copy launch."""
+
+    def __init__(self, n_pages, page_size=16):
+        super().__init__(1, 1, 32, n_pages=n_pages, page_size=page_size, device="cpu")
+        self.held = [[None] * page_size for _ in range(n_pages)]
+
+    def _copy(self, src, dst):
+        assert not set(src) & set(dst) and len(set(dst)) == len(dst)
+        old = [list(p) for p in self.held]
+        for a, b in zip(src, dst):
+            self.held[b] = old[a]
+
+    def write(self, seq, tokens):
+        batch = self.reserve([seq], len(tokens))
+        assert batch.positions.tolist() == list(range(self.length(seq) - len(tokens), self.length(seq)))
+        for pos, tok in zip(batch.positions.tolist(), tokens):
+            page = int(batch.page_table[0, pos // self.page_size])
+            assert self._refs[page] == 1, "a shared page is written"
+            self.held[page][pos % self.page_size] = tok
+
+    def tokens(self, seq):
+        return [self.held[self._pages[seq][p // self.page_size]][p % self.page_size]
+                for p in range(self.length(seq))]
+
+
+def _consistent(cache):
+    refs = [0] * cache.n_pages
+    for pages in cache._pages.values():
+        for p in pages:
+            refs[p] += 1
+    assert refs == cache._refs
+    assert sorted(cache._free) == [p for p in range(cache.n_pages) if refs[p] == 0]
+
+
+def test_padded_head_dim():
+    assert [padded_head_dim(d) for d in (1, 32, 33, 64, 65, 128, 129, 256)] == [32, 32, 64, 64, 128,
+                                                                               128, 256, 256]
+    for bad in (0, -1, 257):
+        with pytest.raises(ValueError, match="head_dim"):
+            padded_head_dim(bad)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_forks_truncations_and_compactions_keep_tokens(seed):
+    rng = random.Random(seed)
+    cache = _ListCache(96)
+    expected = {}
+    for step in range(400):
+        op = rng.choice(["new", "write", "write", "write", "fork", "truncate", "free", "compact"])
+        seqs = list(expected)
+        if op == "new" or not seqs:
+            expected[cache.new_sequence()] = []
+        elif op == "write":
+            s = rng.choice(seqs)
+            toks = [(step, i) for i in range(rng.choice([0, 1, 1, 5, 16, 33]))]
+            before = cache.free_pages
+            try:
+                cache.write(s, toks)
+                expected[s] += toks
+            except RuntimeError as e:
+                assert "free" in str(e) and cache.free_pages == before
+        elif op == "fork":
+            s = rng.choice(seqs)
+            expected[cache.fork(s)] = list(expected[s])
+        elif op == "truncate":
+            s = rng.choice(seqs)
+            n = rng.randint(0, len(expected[s]))
+            cache.truncate(s, n)
+            del expected[s][n:]
+        elif op == "free":
+            s = rng.choice(seqs)
+            cache.free(s)
+            del expected[s]
+        else:
+            cache.compact()
+            used = [p for p in range(cache.n_pages) if cache._refs[p]]
+            assert used == list(range(len(used)))
+            assert cache.compact() == 0
+        _consistent(cache)
+    for s, toks in expected.items():
+        assert cache.tokens(s) == toks
+
+
+def test_batch_of_forks_copies_each_shared_page_but_once_left():
+    cache = _ListCache(8)
+    a = cache.new_sequence()
+    cache.write(a, list(range(20)))
+    b, c = cache.fork(a), cache.fork(a)
+    assert cache.free_pages == 6
+    batch = cache.reserve([a, b, c], 1)
+    # two of the three copy the half-filled page, the last keeps it; the full page stays shared
+    assert cache.free_pages == 4
+    table = batch.page_table.tolist()
+    assert len({row[0] for row in table}) == 1 and len({row[1] for row in table}) == 3
+    assert batch.kv_lens.tolist() == [21] * 3 and batch.cu_tokens.tolist() == [0, 1, 2, 3]
+
+
+def test_reserve_refusals_change_nothing():
+    cache = _ListCache(2)
+    a, b = cache.new_sequence(), cache.new_sequence()
+    cache.write(a, [1] * 16)
+    with pytest.raises(RuntimeError, match="2 pages needed, 1 free"):
+        cache.reserve([a, b], 1)
+    assert cache.length(a) == 16 and cache.length(b) == 0 and cache.free_pages == 1
+    with pytest.raises(ValueError, match="each sequence once"):
+        cache.reserve([a, a], 1)
+    with pytest.raises(ValueError, match=">= 0"):
+        cache.reserve([a], [-1])
+    with pytest.raises(ValueError, match="one count"):
+        cache.reserve([a, b], [1])
+    with pytest.raises(KeyError):
+        cache.reserve([99], 1)
+    with pytest.raises(ValueError, match="truncate"):
+        cache.truncate(a, 17)
+    cache.free(a)
+    with pytest.raises(KeyError):
+        cache.length(a)
+
+
+def test_constructor_refusals():
+    for kw, match in [(dict(n_pages=0), "positive"), (dict(n_pages=1, page_size=24), "page_size")]:
+        with pytest.raises(ValueError, match=match):
+            PagedKVCache(1, 1, 64, device="cpu", **kw)
+    with pytest.raises(ValueError, match="head_dim"):
+        PagedKVCache(1, 1, 300, n_pages=1, device="cpu")
+
+
+def test_operators_require_cuda():
+    codes, scales = torch.zeros(2, 2, 1, 16, 32, dtype=torch.int8), torch.zeros(2, 2, 1, 1)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    cu = torch.tensor([0, 1], dtype=torch.int32)
+    x = torch.zeros(1, 1, 32)
+    with pytest.raises(RuntimeError, match="requires CUDA"):
+        kv_cache.kv_append(codes, scales, table, lens, cu, x, x)
+    with pytest.raises(RuntimeError, match="requires CUDA"):
+        kv_cache.kv_attention(x, codes, scales, table, lens, cu)
+    with pytest.raises(RuntimeError, match="requires CUDA"):
+        kv_cache.kv_read(codes, scales, table, lens, cu, 1)
+    with pytest.raises(RuntimeError, match="requires CUDA"):
+        kv_cache.kv_copy_pages(codes[None], scales[None], lens, lens)
+
+
+def test_c_entries_refuse_bad_arguments_without_a_launch():
+    """Status codes straight from the library: nothing is launched, so no GPU is needed."""
+    from local_ai_training_b200 import _lib
+
+    lib = _lib.lib()
+
+    def attention(page=64, dim=128, hd=128, dtype=1, qh=8, kvh=8, pages=4, tokens=1, seqs=1, scale=1.0,
+                  codes=16):
+        return lib.rt_kv_attention(16, dtype, 1, 1, qh, hd, codes, 16, pages, kvh, page, dim, 16, 1,
+                                   16, 16, seqs, tokens, scale, 16, 1, 1, None, 0, None)
+
+    for kw, kind, match in [
+            (dict(page=24), ValueError, "page_size"), (dict(page=512), ValueError, "page_size"),
+            (dict(dim=96), ValueError, "padded head width"), (dict(hd=129), ValueError, "head_dim"),
+            (dict(hd=0), ValueError, "head_dim"), (dict(dtype=2), TypeError, "float32 or bfloat16"),
+            (dict(qh=9), ValueError, "multiple of kv heads"), (dict(pages=0), ValueError, "cache shape"),
+            (dict(codes=8), ValueError, "16-byte aligned"), (dict(tokens=-1), ValueError, "negative"),
+            (dict(seqs=1 << 21), RuntimeError, "too large"),
+            (dict(scale=float("nan")), ValueError, "finite"),
+            (dict(scale=float("inf")), ValueError, "finite")]:
+        with pytest.raises(kind, match=match):
+            _lib.check(attention(**kw))
+    with pytest.raises(TypeError, match="kv_append"):
+        _lib.check(lib.rt_kv_append(16, 16, 1, 1, 16, 32, 16, 1, 16, 16, 1, 1, 16, 16, 2, 32, 1, 1, 1, 1,
+                                    None))
+    with pytest.raises(TypeError, match="kv_read"):
+        _lib.check(lib.rt_kv_read(16, 16, 1, 1, 16, 32, 16, 1, 16, 16, 1, 1, 32, 16, 16, 3, None))
+    with pytest.raises(ValueError, match="null pointer"):
+        _lib.check(lib.rt_kv_copy_pages(16, 16, 1, 4, 1, 16, 32, None, 16, 1, None, 0, None))
+    with pytest.raises(RuntimeError, match="more pairs"):
+        _lib.check(lib.rt_kv_copy_pages(16, 16, 1, 4, 1, 16, 32, 16, 16, 5, None, 0, None))
