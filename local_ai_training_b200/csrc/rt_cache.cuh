@@ -236,78 +236,6 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvCopy a, int copy_blocks)
   for (int64_t i = threadIdx.x; i < a.page_scales; i += blockDim.x) st[i] = sf[i];
 }
 
-// ------------------------------------------------------------------------------------------
-// Causal attention of the newest tokens over the cache: query row i of a sequence sits at position
-// start + i and sees the keys at positions <= its own.
-//   o = sum_j exp2(t_j - m) · sv_j · V_j / sum_j exp2(t_j - m),  t_j = scale · log2(e) · sk_j · (q · K_j)
-// A row that sees no key is zero, as is a row of no sequence.
-// ------------------------------------------------------------------------------------------
-struct KvAttn {
-  const void *q;
-  int64_t q_token, q_head;
-  void *out;
-  int64_t o_token, o_head;
-  int q_heads, head_dim;
-  float scale_log2;  // softmax scale · log2(e)
-};
-
-// One warp per (row, query head); lanes over the head's width.
-template <typename T>
-__global__ void __launch_bounds__(256) kv_attention_row_kernel(KvCache c, KvBatch b, KvAttn a) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t t = w / a.q_heads;
-  const int h = static_cast<int>(w % a.q_heads), kvh = h / (a.q_heads / c.kv_heads);
-  if (t >= b.n_tokens) return;
-  const T *q = static_cast<const T *>(a.q) + t * a.q_token + h * a.q_head;
-  T *o = static_cast<T *>(a.out) + t * a.o_token + h * a.o_head;
-  float qv[8], acc[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    qv[i] = d < a.head_dim ? load_as_float(q + d) : 0.0f;
-    acc[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  const int64_t s = kv_seq_of(b.cu, b.n_seqs, t);
-  int seen = 0;
-  if (s >= 0) {
-    const KvSeq sq = kv_seq(b, c.page_size, s);
-    seen = min(sq.start + static_cast<int>(t) - sq.c0 + 1, sq.len);
-  }
-  for (int blk = 0; blk * KV_BLOCK < seen; ++blk) {
-    const int64_t page = kv_page(c, b, s, blk);
-    if (page < 0) continue;
-    const int in_page = blk & ((c.page_size >> 4) - 1);
-    const int8_t *kp = c.block(page, 0, kvh, in_page), *vp = c.block(page, 1, kvh, in_page);
-    const float sk = *c.scale(page, 0, kvh, in_page) * a.scale_log2;
-    const float sv = *c.scale(page, 1, kvh, in_page);
-    const int rows = min(KV_BLOCK, seen - blk * KV_BLOCK);
-    for (int r = 0; r < rows; ++r) {
-      float dot = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < c.dim) dot += qv[i] * static_cast<float>(kp[r * c.dim + lane + 32 * i]);
-      const float x = warp_sum_butterfly(dot) * sk;
-      const float mn = fmaxf(m, x), f = exp2f(m - mn), p = exp2f(x - mn);
-      l = l * f + p;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < c.dim)
-          acc[i] = acc[i] * f + p * sv * static_cast<float>(vp[r * c.dim + lane + 32 * i]);
-      m = mn;
-    }
-  }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    if (d < a.head_dim) store_from_float(o + d, acc[i] * inv);
-  }
-}
-
 // Shared argument checks of the cache entry points; 0 or the failure's status.
 inline int kv_check(const char *what, const void *codes, const void *scales, int64_t n_pages,
                     int64_t kv_heads, int64_t page_size, int64_t dim, int64_t head_dim,
@@ -432,50 +360,4 @@ extern "C" int rt_kv_copy_pages(void *codes, float *scales, int64_t layers, int6
   launch_k(kv_copy_kernel, static_cast<unsigned>(blocks + table_blocks), 256, 0, as_stream(stream),
            a, static_cast<int>(blocks));
   return check_launch("kv_copy_pages");
-}
-
-extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
-                                                   int64_t kv_heads, int64_t padded_dim) {
-  (void)n_seqs, (void)n_tokens, (void)q_heads, (void)kv_heads, (void)padded_dim;
-  return 0;
-}
-
-extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
-                               int64_t q_stride_head, int64_t q_heads, int64_t head_dim,
-                               const void *codes, const float *scales, int64_t n_pages,
-                               int64_t kv_heads, int64_t page_size, int64_t padded_dim,
-                               const int32_t *page_table, int64_t pages_per_seq,
-                               const int32_t *kv_lens, const int32_t *cu_tokens, int64_t n_seqs,
-                               int64_t n_tokens, double softmax_scale, void *out,
-                               int64_t o_stride_token, int64_t o_stride_head, void *workspace,
-                               int64_t workspace_bytes, void *stream) {
-  KvCache c;
-  KvBatch b;
-  if (int rc = kv_check("kv_attention", codes, scales, n_pages, kv_heads, page_size, padded_dim,
-                        head_dim, &c))
-    return rc;
-  if (int rc = kv_check_batch("kv_attention", page_table, pages_per_seq, kv_lens, cu_tokens, n_seqs,
-                              n_tokens, page_size, &b))
-    return rc;
-  if (dtype != RT_F32 && dtype != RT_BF16)
-    return fail(RT_ERR_DTYPE, "kv_attention: queries must be float32 or bfloat16");
-  if (q_heads <= 0 || q_heads % kv_heads != 0)
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: query heads must be a multiple of kv heads");
-  if (!(softmax_scale == softmax_scale) || softmax_scale - softmax_scale != 0)
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: softmax scale must be finite");
-  if (n_tokens == 0) return RT_OK;
-  if (q == nullptr || out == nullptr)
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: null pointer");
-  (void)workspace, (void)workspace_bytes;
-  const KvAttn a{q, q_stride_token, q_stride_head, out, o_stride_token, o_stride_head,
-                 static_cast<int>(q_heads), static_cast<int>(head_dim),
-                 static_cast<float>(softmax_scale * 1.4426950408889634)};
-  const int64_t grid = (n_tokens * q_heads + 7) / 8;
-  if (grid > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
-  cudaStream_t s = as_stream(stream);
-  if (dtype == RT_F32)
-    launch_k(kv_attention_row_kernel<float>, static_cast<unsigned>(grid), 256, 0, s, c, b, a);
-  else
-    launch_k(kv_attention_row_kernel<__nv_bfloat16>, static_cast<unsigned>(grid), 256, 0, s, c, b, a);
-  return check_launch("kv_attention");
 }

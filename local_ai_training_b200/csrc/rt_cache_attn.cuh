@@ -1,0 +1,675 @@
+// rt_cache_attn.cuh — causal attention of a batch's newest tokens over the paged int8 cache
+// (rt_cache.cuh), for few query rows per key/value head: single tokens, drafted tokens, and every
+// type and width.
+//
+// Mathematics.  For a query row r (token position p, query head of kv head h) and the keys j <= p:
+//   t_j = (softmax_scale · log2 e · sk_b) (q_r · K_j)   K_j int8 codes, sk_b, sv_b the scales of j's block
+//   o_r = sum_j 2^(t_j - m) sv_b V_j / sum_j 2^(t_j - m)
+// in one pass with a running m.  An int8 code is exact in bf16, so both products run on the tensor
+// cores and accumulate in fp32.  The weight 2^(t - m)·sv is split into two bf16 parts (16 bits: one
+// part alone rounds many equal weights the same way, which does not average out over few rows and
+// narrow heads); for fp32 queries q and the weights are split into three, all 24 bits.
+//
+// Layout of one warp's step, 16 keys (one quantisation block), no shared-memory transposes:
+//   S^T (16 keys x 8 rows) = K (m16 x k16) · q^T:  lane (g, t) = (lane / 4, lane % 4) holds keys g and
+//     g + 8 and takes 16 consecutive bytes of each row; the k index of the product is any order of
+//     the head's width, so those 16 bytes are four k-steps' operands and q is laid out to match.
+//   O^T (D x 8 rows) += V^T (m16 dims x k16 keys) · P^T:  the m index is any order of the width too: lane
+//     (g, t) takes D / 8 consecutive bytes of keys 2t, 2t+1, 2t+8, 2t+9; byte permutes pair the keys.
+//   P^T's operand is S^T's accumulator transposed within the warp (movmatrix).
+// Each lane copies exactly the bytes it will use (cp.async, its own slots), so a warp's ring of
+// stages needs no barrier.
+//
+// Work split: the key blocks of all (sequence, row tile, kv head) units are one line, cut into equal
+// pieces, one per CTA; the eight warps of a CTA take its blocks in turn and merge in shared memory.
+// A unit cut by a CTA's end leaves partial (m, l, O) rows in the workspace, which a second launch
+// joins in CTA order.  Lengths are read on the device; a long sequence, a ragged batch and many
+// short sequences all load every SM alike.
+#pragma once
+
+#include "rt_cache.cuh"
+
+namespace rt {
+
+constexpr int KA_WARPS = 8;
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two int8 in the 16-bit lanes' low bytes under 0x43 -> two bf16, exact.  0x43bb as bf16 is
+// 128 + low7(b), and the sign bit of b, left in place, turns the subtrahend 128 into 256.
+__device__ __forceinline__ uint32_t bf16x2_of_43(uint32_t w) {
+  const uint32_t a = w & 0xFF7FFF7Fu, s = w & 0xFF80FF80u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+                                   *reinterpret_cast<const __nv_bfloat162 *>(&s));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+// bytes 0, 1 (hi = false) or 2, 3 of w -> bf16x2
+template <bool HI>
+__device__ __forceinline__ uint32_t bf16x2_of_bytes(uint32_t w) {
+  return bf16x2_of_43(__byte_perm(w, 0x43434343u, HI ? 0x4342 : 0x4140));
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_async_ca(uint32_t smem, const void *gmem) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem), "l"(gmem), "n"(BYTES)
+                 : "memory");
+}
+// x as `parts` bf16 values whose sum is x to 8·parts bits; part i of two values, packed
+template <int PARTS>
+__device__ __forceinline__ void split_bf16x2(float x, float y, uint32_t (&p)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    p[i] = pack_bf16x2(x, y);
+    if (i + 1 < PARTS) {
+      x = __fsub_rn(x, __uint_as_float(p[i] << 16));
+      y = __fsub_rn(y, __uint_as_float(p[i] & 0xFFFF0000u));
+    }
+  }
+}
+
+struct KvAttn {
+  const void *q;
+  int64_t q_token, q_head;
+  void *out;
+  int64_t o_token, o_head;
+  int q_heads, group, head_dim;
+  float scale_log2;  // softmax scale · log2(e)
+  bool q_vec;        // q rows allow 16-byte loads of whole stored widths
+  float *ws;         // partial rows: [2 · grid][RT][D + 2]
+  int4 *meta;        // per CTA: {sequence or -1, row tile, kv head, head slot ends its unit}
+};
+
+// Walks the line of (sequence, row tile, kv head) units from a CTA's first block on.
+template <int RT>
+struct KvWalk {
+  int s, tile, head;       // unit
+  int b, e, nb;            // piece [b, e) of the unit's nb blocks
+  int left;                // blocks of the CTA from b on
+  KvSeq q;
+  int tiles;
+
+  __device__ __forceinline__ void set_tile(int group) {
+    const int rows = min((tile + 1) * RT, q.n * group);
+    const int seen = min(max(q.start + (rows - 1) / group + 1, 0), q.len);
+    nb = max((seen + KV_BLOCK - 1) / KV_BLOCK, 1);
+  }
+  __device__ __forceinline__ void set_seq(const KvCache &c, const KvBatch &bt, int group) {
+    q = kv_seq(bt, c.page_size, s);
+    tiles = (q.n * group + RT - 1) / RT;
+  }
+  // the unit after this one (none: left = 0)
+  __device__ __forceinline__ void next(const KvCache &c, const KvBatch &bt, int group) {
+    left -= e - b;
+    if (left <= 0) return;
+    if (++head == c.kv_heads) {
+      head = 0;
+      if (++tile >= tiles) {
+        tile = 0;
+        do {
+          if (++s >= bt.n_seqs) {
+            left = 0;
+            return;
+          }
+          set_seq(c, bt, group);
+        } while (tiles == 0);
+      }
+      set_tile(group);
+    }
+    b = 0;
+    e = min(nb, left);
+  }
+};
+
+// Blocks of sequence s over all its row tiles (one kv head).
+template <int RT>
+__device__ __forceinline__ int64_t kv_seq_blocks(const KvCache &c, const KvBatch &bt, int group, int s) {
+  KvWalk<RT> w;
+  w.s = s;
+  w.set_seq(c, bt, group);
+  int64_t sum = 0;
+  for (w.tile = 0; w.tile < w.tiles; ++w.tile) {
+    w.set_tile(group);
+    sum += w.nb;
+  }
+  return sum;
+}
+
+template <typename T, int D, int NT>
+struct KaShape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int PARTS = F32 ? 3 : 1;              // bf16 parts of q
+  static constexpr int WP = F32 ? 3 : 2;                 // bf16 parts of a weight
+  static constexpr int RT = 8 * NT;
+  static constexpr int KS = D / 16;                      // k-steps of q·K, m-tiles of V·p
+  static constexpr int KCH = D >= 64 ? D / 64 : 1;       // K chunks of a row per lane
+  static constexpr int KB = D >= 64 ? 16 : 8;            // their bytes
+  static constexpr int VCH = D >= 128 ? D / 128 : 1;     // V chunks of a key per lane
+  static constexpr int VB = D >= 128 ? 16 : D / 8;       // their bytes
+  static constexpr int STAGE = 2 * 16 * D + 16;          // bytes of a stage of one warp, scales last
+  static constexpr int STAGES = D >= 256 || (D == 128 && NT == 1 && !F32) ? 2 : 4;
+  static constexpr int RING = KA_WARPS * STAGES * STAGE;
+  static constexpr int OP = D + 4;                       // floats of a merged row
+  static constexpr int MERGE = KA_WARPS * RT * (OP + 2) * 4;
+  static constexpr int SMEM = RING + MERGE;
+  static constexpr int MIN_CTAS = NT == 1 && D <= 128 && !F32 ? 2 : 1;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
+    kv_attention_kernel(KvCache c, KvBatch bt, KvAttn a, int min_blocks) {
+  using SH = KaShape<T, D, NT>;
+  constexpr int RT = SH::RT, KS = SH::KS, PARTS = SH::PARTS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t sm_sum[KA_WARPS];
+  __shared__ int sm_start[4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- rows of no sequence
+  {
+    const int64_t first = bt.n_seqs > 0 ? max(min(static_cast<int64_t>(bt.cu[bt.n_seqs]), bt.n_tokens),
+                                              static_cast<int64_t>(0))
+                                        : 0;
+    const int64_t n = (bt.n_tokens - first) * a.q_heads * a.head_dim;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + tid; i < n;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+      const int64_t r = i / a.head_dim;
+      store_from_float(static_cast<T *>(a.out) + (first + r / a.q_heads) * a.o_token +
+                           (r % a.q_heads) * a.o_head + i % a.head_dim,
+                       0.0f);
+    }
+  }
+
+  // ---- this CTA's piece of the line of blocks
+  KvWalk<RT> w;
+  {
+    const int per = static_cast<int>((bt.n_seqs + KA_WARPS * 32 - 1) / (KA_WARPS * 32));
+    const int s0 = min(tid * per, static_cast<int>(bt.n_seqs));
+    const int s1 = min(s0 + per, static_cast<int>(bt.n_seqs));
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += kv_seq_blocks<RT>(c, bt, a.group, s);
+    mine *= c.kv_heads;
+    int64_t scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) sm_sum[warp] = scan;
+    if (tid == 0) sm_start[0] = -1;
+    __syncthreads();
+    int64_t before = scan - mine, total = 0;
+#pragma unroll
+    for (int i = 0; i < KA_WARPS; ++i) {
+      if (i < warp) before += sm_sum[i];
+      total += sm_sum[i];
+    }
+    // as many CTAs as have min_blocks each, all of the grid when the line is long
+    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + min_blocks - 1) / min_blocks);
+    const int64_t p0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+    const int64_t p1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+    if (p0 < p1 && before <= p0 && p0 < before + mine) {
+      int64_t at = before;
+      for (w.s = s0; w.s < s1 - 1; ++w.s) {
+        const int64_t n = kv_seq_blocks<RT>(c, bt, a.group, w.s) * c.kv_heads;
+        if (p0 < at + n) break;
+        at += n;
+      }
+      w.set_seq(c, bt, a.group);
+      for (w.tile = 0;; ++w.tile) {
+        w.set_tile(a.group);
+        const int64_t n = static_cast<int64_t>(w.nb) * c.kv_heads;
+        if (p0 < at + n || w.tile >= w.tiles - 1) break;
+        at += n;
+      }
+      sm_start[0] = w.s, sm_start[1] = w.tile;
+      sm_start[2] = static_cast<int>((p0 - at) / w.nb), sm_start[3] = static_cast<int>((p0 - at) % w.nb);
+    }
+    __syncthreads();
+    if (sm_start[0] < 0) {
+      if (tid == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+    w.s = sm_start[0], w.tile = sm_start[1], w.head = sm_start[2], w.b = sm_start[3];
+    w.left = static_cast<int>(p1 - p0);
+    w.set_seq(c, bt, a.group);
+    w.set_tile(a.group);
+    w.e = min(w.nb, w.b + w.left);
+  }
+
+  // ---- loads: a second walk, STAGES - 1 blocks of this warp ahead
+  const uint32_t ring = smem_u32(smem) + warp * SH::STAGES * SH::STAGE;
+  KvWalk<RT> ld = w;
+  int ld_blk = ld.b + warp;  // this warp's next block
+  const auto ld_settle = [&] {  // moves on to the piece that holds this warp's next block
+    while (ld.left > 0 && ld_blk >= ld.e) {
+      ld.next(c, bt, a.group);
+      ld_blk = ld.b + warp;
+    }
+  };
+  const int koff = g * D + t4 * SH::KB;
+  const int voff = (D >= 128 ? g * 16 : g * SH::VB) + 2 * t4 * D;
+  const int64_t part = static_cast<int64_t>(c.kv_heads) * c.page_size * D;
+  const auto fetch = [&](int stage) {
+    ld_settle();
+    if (ld.left > 0) {
+      const uint32_t st = ring + stage * SH::STAGE;
+      const int64_t page = ld_blk * KV_BLOCK < ld.q.len ? kv_page(c, bt, ld.s, ld_blk) : -1;
+      const int in_page = ld_blk & ((c.page_size >> 4) - 1);
+      if (page >= 0) {
+        const int8_t *kp = c.block(page, 0, ld.head, in_page);
+        const int8_t *vp = kp + part;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < SH::KCH; ++j)
+            cp_async_ca<SH::KB>(st + ((r * SH::KCH + j) * 32 + lane) * SH::KB,
+                                kp + koff + r * 8 * D + j * 64);
+        const uint32_t sv = st + 16 * D;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < SH::VCH; ++j)
+            cp_async_ca<SH::VB>(sv + ((r * SH::VCH + j) * 32 + lane) * SH::VB,
+                                vp + voff + ((r & 1) + (r >> 1) * 8) * D + j * 128);
+        if (lane < 2)
+          cp_async_ca<4>(st + 32 * D + lane * 4, c.scale(page, lane, ld.head, in_page));
+      }
+      if (lane == 2)
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(st + 32 * D + 8), "r"(page >= 0 ? 1 : 0) : "memory");
+      ld_blk += KA_WARPS;
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < SH::STAGES - 1; ++i) fetch(i);
+
+  float *merge = reinterpret_cast<float *>(smem + SH::RING);
+  float *merge_ml = merge + KA_WARPS * RT * SH::OP;
+  int stage = 0;
+  bool first_piece = true;
+  while (w.left > 0) {
+    // ---- query rows as the products' B operand: lane (g, t) holds row g's bytes of lane t
+    const int row0 = w.tile * RT, rows = min(RT, w.q.n * a.group - row0);
+    uint32_t qf[NT][KS][2][PARTS];
+    int lim[NT][2];  // keys that rows 2t and 2t + 1 see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + n * 8 + g;
+      const bool in = n * 8 + g < rows;
+      const T *qp = static_cast<const T *>(a.q) +
+                    (w.q.c0 + static_cast<int64_t>(in ? r / a.group : 0)) * a.q_token +
+                    static_cast<int64_t>(w.head * a.group + (in ? r % a.group : 0)) * a.q_head;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        // k-step j: the 4 bytes 4 (j % 4) .. of chunk j / 4 (of 64 wide, or 8 bytes of 32)
+        const int d = D >= 64 ? (j >> 2) * 64 + t4 * 16 + (j & 3) * 4 : t4 * 8 + j * 4;
+        float x[4];
+        if (a.q_vec && in) {
+          if constexpr (SH::F32) {
+            const float4 v = *reinterpret_cast<const float4 *>(qp + d);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(qp + d);
+            x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+            x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xFFFF0000u);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = in && d + i < a.head_dim ? load_as_float(qp + d + i) : 0.0f;
+        }
+        split_bf16x2<PARTS>(x[0], x[1], qf[n][j][0]);
+        split_bf16x2<PARTS>(x[2], x[3], qf[n][j][1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int tok = (row0 + min(n * 8 + 2 * t4 + e, rows - 1)) / a.group;
+        lim[n][e] = min(w.q.start + tok + 1, w.q.len);
+      }
+    }
+    const int lim_all = min(w.q.start + row0 / a.group + 1, w.q.len);  // keys that every row sees
+
+    float o[NT][KS][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[n][i][x] = 0.0f;
+      m[n][0] = m[n][1] = -1e30f;  // finite: a masked score of -inf under it weighs 0, not NaN
+      l[n][0] = l[n][1] = 0.0f;
+    }
+
+    for (int blk = w.b + warp; blk < w.e; blk += KA_WARPS) {
+      __syncwarp();  // the stage about to be refilled has been read by every lane
+      fetch(stage == 0 ? SH::STAGES - 1 : stage - 1);
+      cp_async_wait<SH::STAGES - 1>();
+      __syncwarp();
+      const uint8_t *st = smem + (warp * SH::STAGES + stage) * SH::STAGE;
+      stage = stage + 1 == SH::STAGES ? 0 : stage + 1;
+      const float *sc = reinterpret_cast<const float *>(st + 32 * D);
+      if (reinterpret_cast<const int *>(sc)[2] == 0) continue;  // no page: no keys
+      const float sk = sc[0] * a.scale_log2, sv = sc[1];
+
+      // ---- S^T = K · q^T
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < SH::KCH; ++j) {
+        uint32_t k0[4], k1[4];
+        if constexpr (SH::KB == 16) {
+          const uint4 u = *reinterpret_cast<const uint4 *>(st + (j * 32 + lane) * 16);
+          const uint4 v = *reinterpret_cast<const uint4 *>(st + ((SH::KCH + j) * 32 + lane) * 16);
+          k0[0] = u.x, k0[1] = u.y, k0[2] = u.z, k0[3] = u.w;
+          k1[0] = v.x, k1[1] = v.y, k1[2] = v.z, k1[3] = v.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2 *>(st + lane * 8);
+          const uint2 v = *reinterpret_cast<const uint2 *>(st + (32 + lane) * 8);
+          k0[0] = u.x, k0[1] = u.y, k1[0] = v.x, k1[1] = v.y;
+        }
+#pragma unroll
+        for (int i = 0; i < SH::KB / 4; ++i) {
+          const uint32_t af[4] = {bf16x2_of_bytes<false>(k0[i]), bf16x2_of_bytes<false>(k1[i]),
+                                  bf16x2_of_bytes<true>(k0[i]), bf16x2_of_bytes<true>(k1[i])};
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int p = PARTS - 1; p >= 0; --p)  // small parts first
+              mma_bf16(s[n], af, qf[n][j * 4 + i][0][p], qf[n][j * 4 + i][1][p]);
+        }
+      }
+
+      // ---- scores in units of log2, masked, against the running maximum.  The maximum moves only when
+      // a score exceeds it by 2^6: weights stay below 64, and most steps need one vote instead of
+      // the reduction over the keys.
+      const int key0 = blk * KV_BLOCK + g;
+      const bool cut = (blk + 1) * KV_BLOCK > lim_all;
+      bool up = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          s[n][x] *= sk;
+          if (cut && key0 + (x >> 1) * 8 >= lim[n][x & 1]) s[n][x] = -INFINITY;
+          up |= s[n][x] > m[n][x & 1] + 6.0f;
+        }
+      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = fmaxf(s[n][e], s[n][e + 2]);
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            const float mn = fmaxf(m[n][e], v), f = ex2(m[n][e] - mn);
+            m[n][e] = mn;
+            l[n][e] *= f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) o[n][i][e] *= f, o[n][i][e + 2] *= f;
+          }
+      }
+      uint32_t pf[NT][2][SH::WP];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float p[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          p[x] = ex2(s[n][x] - m[n][x & 1]);
+          l[n][x & 1] += p[x];
+          p[x] *= sv;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          split_bf16x2<SH::WP>(p[2 * e], p[2 * e + 1], pf[n][e]);
+#pragma unroll
+          for (int i = 0; i < SH::WP; ++i) pf[n][e][i] = movmatrix_trans(pf[n][e][i]);
+        }
+      }
+
+      // ---- O^T += V^T · P^T
+      const uint8_t *vs = st + 16 * D;
+#pragma unroll
+      for (int j = 0; j < SH::VCH; ++j) {
+        uint32_t v[4][SH::VB / 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint8_t *at = vs + ((r * SH::VCH + j) * 32 + lane) * SH::VB;
+          if constexpr (SH::VB == 16) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(at);
+            v[r][0] = u.x, v[r][1] = u.y, v[r][2] = u.z, v[r][3] = u.w;
+          } else if constexpr (SH::VB == 8) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(at);
+            v[r][0] = u.x, v[r][1] = u.y;
+          } else {
+            v[r][0] = *reinterpret_cast<const uint32_t *>(at);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < SH::VB / 4; ++i) {
+          // (key 2t, key 2t+1) byte pairs of four dims, then keys 2t+8, 2t+9
+          const uint32_t lo01 = __byte_perm(v[0][i], v[1][i], 0x5140);
+          const uint32_t lo23 = __byte_perm(v[0][i], v[1][i], 0x7362);
+          const uint32_t hi01 = __byte_perm(v[2][i], v[3][i], 0x5140);
+          const uint32_t hi23 = __byte_perm(v[2][i], v[3][i], 0x7362);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t lo = x ? lo23 : lo01, hi = x ? hi23 : hi01;
+            const uint32_t af[4] = {bf16x2_of_bytes<false>(lo), bf16x2_of_bytes<true>(lo),
+                                    bf16x2_of_bytes<false>(hi), bf16x2_of_bytes<true>(hi)};
+            const int mt = j * (SH::VB / 2) + i * 2 + x;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int p = SH::WP - 1; p >= 0; --p) mma_bf16(o[n][mt], af, pf[n][0][p], pf[n][1][p]);
+          }
+        }
+      }
+    }
+
+    // ---- merge the warps: rows' maxima, then the rescaled rows, summed in warp order
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+        const int r = n * 8 + 2 * t4 + e;
+        if (g == 0) merge_ml[(warp * RT + r) * 2] = m[n][e], merge_ml[(warp * RT + r) * 2 + 1] = l[n][e];
+        if (r < rows) {
+          float *dst = merge + (warp * RT + r) * SH::OP;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const int d = D >= 128 ? (i >> 3) * 128 + g * 16 + (i & 7) * 2 : g * (D / 8) + i * 2;
+            *reinterpret_cast<float2 *>(dst + d) = make_float2(o[n][i][e], o[n][i][e + 2]);
+          }
+        }
+      }
+    __syncthreads();
+    const bool whole = w.b == 0 && w.e == w.nb;
+    const int slot = blockIdx.x * 2 + (w.b > 0 ? 0 : 1);
+    for (int i = tid; i < rows * D; i += KA_WARPS * 32) {
+      const int r = i / D, d = i % D;
+      float top = -1e30f;
+#pragma unroll
+      for (int x = 0; x < KA_WARPS; ++x) top = fmaxf(top, merge_ml[(x * RT + r) * 2]);
+      float sum = 0.0f, den = 0.0f;
+#pragma unroll
+      for (int x = 0; x < KA_WARPS; ++x) {
+        const float f = ex2(merge_ml[(x * RT + r) * 2] - top);
+        den += f * merge_ml[(x * RT + r) * 2 + 1];
+        sum += f * merge[(x * RT + r) * SH::OP + d];
+      }
+      if (whole) {
+        if (d < a.head_dim) {
+          const int tok = (row0 + r) / a.group, h = w.head * a.group + (row0 + r) % a.group;
+          store_from_float(static_cast<T *>(a.out) + (w.q.c0 + static_cast<int64_t>(tok)) * a.o_token +
+                               static_cast<int64_t>(h) * a.o_head + d,
+                           den > 0.0f ? __fdividef(sum, den) : 0.0f);
+        }
+      } else {
+        float *dst = a.ws + (static_cast<int64_t>(slot) * RT + r) * (D + 2);
+        dst[2 + d] = sum;
+        if (d == 0) dst[0] = top, dst[1] = den;
+      }
+    }
+    if (tid == 0) {
+      int4 *mt = a.meta + blockIdx.x;
+      if (first_piece) *mt = make_int4(-1, 0, 0, 0);
+      if (w.b > 0) mt->w = w.e == w.nb;
+      if (w.b == 0 && !whole) mt->x = w.s, mt->y = w.tile, mt->z = w.head;
+    }
+    first_piece = false;
+    __syncthreads();
+    w.next(c, bt, a.group);
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the partial rows of every unit that a CTA began and did not end: its own, then those of the
+// following CTAs up to the one that ended the unit.
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBatch bt, KvAttn a, int ctas) {
+  pdl_wait();
+  pdl_trigger();
+  const int4 mt = a.meta[blockIdx.x];
+  if (mt.x < 0) return;
+  int last = blockIdx.x + 1;
+  while (last < ctas - 1 && a.meta[last].w == 0) ++last;
+  const KvSeq q = kv_seq(bt, c.page_size, mt.x);
+  const int row0 = mt.y * RT, rows = min(RT, q.n * a.group - row0);
+  const auto slot = [&](int cta, int r) {
+    return a.ws + (static_cast<int64_t>(cta * 2 + (cta == static_cast<int>(blockIdx.x))) * RT + r) * (D + 2);
+  };
+  for (int i = threadIdx.x; i < rows * D; i += 256) {
+    const int r = i / D, d = i % D;
+    float top = -1e30f;
+    for (int x = blockIdx.x; x <= last; ++x) top = fmaxf(top, slot(x, r)[0]);
+    float sum = 0.0f, den = 0.0f;
+    for (int x = blockIdx.x; x <= last; ++x) {
+      const float *p = slot(x, r);
+      const float f = ex2(p[0] - top);
+      den += f * p[1];
+      sum += f * p[2 + d];
+    }
+    if (d < a.head_dim) {
+      const int tok = (row0 + r) / a.group, h = mt.z * a.group + (row0 + r) % a.group;
+      store_from_float(static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(tok)) * a.o_token +
+                           static_cast<int64_t>(h) * a.o_head + d,
+                       den > 0.0f ? __fdividef(sum, den) : 0.0f);
+    }
+  }
+}
+
+inline int kv_sm_count() {
+  int sms = 0;
+  return rt_sm_count(&sms) == RT_OK ? sms : 0;
+}
+constexpr int KA_GRID = 2;  // CTAs per SM at most
+
+template <typename T, int D, int NT>
+int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+  using SH = KaShape<T, D, NT>;
+  auto *kernel = kv_attention_kernel<T, D, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::SMEM);
+  if (e != cudaSuccess) return fail(RT_ERR_CUDA, "kv_attention: %s", cudaGetErrorString(e));
+  const int ctas = sms * SH::MIN_CTAS;
+  launch_k(kernel, ctas, KA_WARPS * 32, SH::SMEM, s, c, bt, a, KA_WARPS);
+  launch_k(kv_attention_join_kernel<T, D, SH::RT>, ctas, 256, 0, s, c, bt, a, ctas);
+  return check_launch("kv_attention");
+}
+template <typename T>
+int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+  // 16-row tiles once the sequences average more than 8 rows per kv head
+  const bool wide = bt.n_tokens * a.group > 8 * bt.n_seqs;
+  switch (c.dim) {
+    case 32:
+      return wide ? kv_attention_run<T, 32, 2>(c, bt, a, sms, s) : kv_attention_run<T, 32, 1>(c, bt, a, sms, s);
+    case 64:
+      return wide ? kv_attention_run<T, 64, 2>(c, bt, a, sms, s) : kv_attention_run<T, 64, 1>(c, bt, a, sms, s);
+    case 128:
+      return wide ? kv_attention_run<T, 128, 2>(c, bt, a, sms, s) : kv_attention_run<T, 128, 1>(c, bt, a, sms, s);
+    default:
+      return kv_attention_run<T, 256, 1>(c, bt, a, sms, s);
+  }
+}
+
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
+                                                   int64_t kv_heads, int64_t padded_dim) {
+  (void)n_seqs, (void)n_tokens, (void)q_heads, (void)kv_heads;
+  const int64_t ctas = static_cast<int64_t>(kv_sm_count()) * KA_GRID;
+  return ctas * 16 + ctas * 2 * 16 * (padded_dim + 2) * 4;
+}
+
+extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
+                               int64_t q_stride_head, int64_t q_heads, int64_t head_dim,
+                               const void *codes, const float *scales, int64_t n_pages,
+                               int64_t kv_heads, int64_t page_size, int64_t padded_dim,
+                               const int32_t *page_table, int64_t pages_per_seq,
+                               const int32_t *kv_lens, const int32_t *cu_tokens, int64_t n_seqs,
+                               int64_t n_tokens, double softmax_scale, void *out,
+                               int64_t o_stride_token, int64_t o_stride_head, void *workspace,
+                               int64_t workspace_bytes, void *stream) {
+  KvCache c;
+  KvBatch b;
+  if (int rc = kv_check("kv_attention", codes, scales, n_pages, kv_heads, page_size, padded_dim,
+                        head_dim, &c))
+    return rc;
+  if (int rc = kv_check_batch("kv_attention", page_table, pages_per_seq, kv_lens, cu_tokens, n_seqs,
+                              n_tokens, page_size, &b))
+    return rc;
+  if (dtype != RT_F32 && dtype != RT_BF16)
+    return fail(RT_ERR_DTYPE, "kv_attention: queries must be float32 or bfloat16");
+  if (q_heads <= 0 || q_heads % kv_heads != 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: query heads must be a multiple of kv heads");
+  if (!(softmax_scale - softmax_scale == 0))
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: softmax scale must be finite");
+  if (n_tokens == 0) return RT_OK;
+  if (q == nullptr || out == nullptr)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: null pointer");
+  if (n_tokens * q_heads > INT32_MAX - 64) return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
+  const int sms = kv_sm_count();
+  if (sms <= 0) return fail(RT_ERR_CUDA, "kv_attention: no device");
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+      workspace_bytes < rt_kv_attention_workspace_bytes(n_seqs, n_tokens, q_heads, kv_heads, padded_dim))
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: workspace too small or not 256-byte aligned");
+  KvAttn a{};
+  a.q = q, a.q_token = q_stride_token, a.q_head = q_stride_head;
+  a.out = out, a.o_token = o_stride_token, a.o_head = o_stride_head;
+  a.q_heads = static_cast<int>(q_heads), a.group = static_cast<int>(q_heads / kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  const int es = dtype == RT_F32 ? 4 : 2;
+  a.q_vec = head_dim == padded_dim && aligned16(q) && (q_stride_token * es) % 16 == 0 &&
+            (q_stride_head * es) % 16 == 0;
+  const int64_t ctas = static_cast<int64_t>(sms) * KA_GRID;
+  a.meta = static_cast<int4 *>(workspace);
+  a.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + ctas * 16);
+  return dtype == RT_F32 ? kv_attention_width<float>(c, b, a, sms, as_stream(stream))
+                         : kv_attention_width<__nv_bfloat16>(c, b, a, sms, as_stream(stream));
+}
