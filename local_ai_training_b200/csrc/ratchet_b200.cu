@@ -5,4 +5,4 @@
 #include "rt_gemm.cuh"
 #include "rt_loss.cuh"
 #include "rt_cache.cuh"
-#include "rt_cache_attn.cuh"
+#include "rt_cache_entry.cuh"

@@ -92,13 +92,15 @@ struct KvAttn {
   int64_t o_token, o_head;
   int q_heads, group, head_dim;
   float scale_log2;  // softmax scale · log2(e)
-  bool q_vec;        // q rows allow 16-byte loads of whole stored widths
+  bool q_vec, o_vec;  // rows of q / out allow 16-byte accesses over the whole stored width
+  int rows_lo, rows_hi;  // this launch takes the sequences with rows_lo <= rows per kv head < rows_hi
   float *ws;         // partial rows: [2 · grid][RT][D + 2]
   int4 *meta;        // per CTA: {sequence or -1, row tile, kv head, head slot ends its unit}
 };
 
-// Walks the line of (sequence, row tile, kv head) units from a CTA's first block on.
-template <int RT>
+// Walks the line of (sequence, row tile, kv head) units from a CTA's first block on.  A unit is RT
+// query rows (token-major, the group's heads innermost) and the blocks of KEYS keys that they see.
+template <int RT, int KEYS>
 struct KvWalk {
   int s, tile, head;       // unit
   int b, e, nb;            // piece [b, e) of the unit's nb blocks
@@ -106,17 +108,30 @@ struct KvWalk {
   KvSeq q;
   int tiles;
 
-  __device__ __forceinline__ void set_tile(int group) {
-    const int rows = min((tile + 1) * RT, q.n * group);
-    const int seen = min(max(q.start + (rows - 1) / group + 1, 0), q.len);
-    nb = max((seen + KV_BLOCK - 1) / KV_BLOCK, 1);
+  // keys that the first `rows` rows of the sequence see
+  __device__ __forceinline__ int seen(const KvAttn &a, int rows) const {
+    return min(max(q.start + (rows - 1) / a.group + 1, 0), q.len);
   }
-  __device__ __forceinline__ void set_seq(const KvCache &c, const KvBatch &bt, int group) {
+  __device__ __forceinline__ void set_tile(const KvAttn &a) {
+    nb = max((seen(a, min((tile + 1) * RT, q.n * a.group)) + KEYS - 1) / KEYS, 1);
+  }
+  __device__ __forceinline__ void set_seq(const KvCache &c, const KvBatch &bt, const KvAttn &a) {
     q = kv_seq(bt, c.page_size, s);
-    tiles = (q.n * group + RT - 1) / RT;
+    const int rows = q.n * a.group;
+    tiles = rows >= a.rows_lo && rows < a.rows_hi ? (rows + RT - 1) / RT : 0;
+  }
+  // Blocks of sequence s over all its row tiles (one kv head).
+  __device__ __forceinline__ int64_t seq_blocks(const KvCache &c, const KvBatch &bt, const KvAttn &a) {
+    set_seq(c, bt, a);
+    int64_t sum = 0;
+    for (tile = 0; tile < tiles; ++tile) {
+      set_tile(a);
+      sum += nb;
+    }
+    return sum;
   }
   // the unit after this one (none: left = 0)
-  __device__ __forceinline__ void next(const KvCache &c, const KvBatch &bt, int group) {
+  __device__ __forceinline__ void next(const KvCache &c, const KvBatch &bt, const KvAttn &a) {
     left -= e - b;
     if (left <= 0) return;
     if (++head == c.kv_heads) {
@@ -128,28 +143,90 @@ struct KvWalk {
             left = 0;
             return;
           }
-          set_seq(c, bt, group);
+          set_seq(c, bt, a);
         } while (tiles == 0);
       }
-      set_tile(group);
+      set_tile(a);
     }
     b = 0;
     e = min(nb, left);
   }
 };
 
-// Blocks of sequence s over all its row tiles (one kv head).
-template <int RT>
-__device__ __forceinline__ int64_t kv_seq_blocks(const KvCache &c, const KvBatch &bt, int group, int s) {
-  KvWalk<RT> w;
-  w.s = s;
-  w.set_seq(c, bt, group);
-  int64_t sum = 0;
-  for (w.tile = 0; w.tile < w.tiles; ++w.tile) {
-    w.set_tile(group);
-    sum += w.nb;
+// Sets this CTA's share of the line: all of the grid has equal shares of a long line, and as many CTAs as
+// get min_blocks each of a short one.  Returns false (for every thread) when this CTA has none.
+template <int THREADS, int RT, int KEYS>
+__device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache &c, const KvBatch &bt,
+                                              const KvAttn &a, int min_blocks) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ int64_t sm_sum[WARPS];
+  __shared__ int sm_start[5];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = static_cast<int>((bt.n_seqs + THREADS - 1) / THREADS);
+  const int s0 = min(tid * per, static_cast<int>(bt.n_seqs));
+  const int s1 = min(s0 + per, static_cast<int>(bt.n_seqs));
+  int64_t mine = 0;
+  for (w.s = s0; w.s < s1; ++w.s) mine += w.seq_blocks(c, bt, a);
+  mine *= c.kv_heads;
+  int64_t scan = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
   }
-  return sum;
+  if (lane == 31) sm_sum[warp] = scan;
+  if (tid == 0) sm_start[0] = -1;
+  __syncthreads();
+  int64_t before = scan - mine, total = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) {
+    if (i < warp) before += sm_sum[i];
+    total += sm_sum[i];
+  }
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + min_blocks - 1) / min_blocks);
+  const int64_t p0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
+  const int64_t p1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
+  if (p0 < p1 && before <= p0 && p0 < before + mine) {  // one thread's sequences hold p0
+    int64_t at = before;
+    for (w.s = s0; w.s < s1 - 1; ++w.s) {
+      const int64_t n = w.seq_blocks(c, bt, a) * c.kv_heads;
+      if (p0 < at + n) break;
+      at += n;
+    }
+    w.set_seq(c, bt, a);
+    for (w.tile = 0;; ++w.tile) {
+      w.set_tile(a);
+      const int64_t n = static_cast<int64_t>(w.nb) * c.kv_heads;
+      if (p0 < at + n || w.tile >= w.tiles - 1) break;
+      at += n;
+    }
+    sm_start[0] = w.s, sm_start[1] = w.tile;
+    sm_start[2] = static_cast<int>((p0 - at) / w.nb), sm_start[3] = static_cast<int>((p0 - at) % w.nb);
+    sm_start[4] = static_cast<int>(p1 - p0);
+  }
+  __syncthreads();
+  if (sm_start[0] < 0) return false;
+  w.s = sm_start[0], w.tile = sm_start[1], w.head = sm_start[2], w.b = sm_start[3];
+  w.left = sm_start[4];
+  w.set_seq(c, bt, a);
+  w.set_tile(a);
+  w.e = min(w.nb, w.b + w.left);
+  return true;
+}
+
+// Zeros for the rows that belong to no sequence (from cu[n_seqs] on).
+template <typename T>
+__device__ __forceinline__ void kv_zero_rest(const KvBatch &bt, const KvAttn &a) {
+  const int64_t end = bt.n_seqs > 0 ? bt.cu[bt.n_seqs] : 0;
+  const int64_t first = max(min(end, bt.n_tokens), static_cast<int64_t>(0));
+  const int64_t n = (bt.n_tokens - first) * a.q_heads * a.head_dim;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = i / a.head_dim;
+    store_from_float(static_cast<T *>(a.out) + (first + r / a.q_heads) * a.o_token +
+                         (r % a.q_heads) * a.o_head + i % a.head_dim,
+                     0.0f);
+  }
 }
 
 template <typename T, int D, int NT>
@@ -178,91 +255,24 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
   using SH = KaShape<T, D, NT>;
   constexpr int RT = SH::RT, KS = SH::KS, PARTS = SH::PARTS;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t sm_sum[KA_WARPS];
-  __shared__ int sm_start[4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   pdl_wait();
   pdl_trigger();
 
-  // ---- rows of no sequence
-  {
-    const int64_t first = bt.n_seqs > 0 ? max(min(static_cast<int64_t>(bt.cu[bt.n_seqs]), bt.n_tokens),
-                                              static_cast<int64_t>(0))
-                                        : 0;
-    const int64_t n = (bt.n_tokens - first) * a.q_heads * a.head_dim;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + tid; i < n;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-      const int64_t r = i / a.head_dim;
-      store_from_float(static_cast<T *>(a.out) + (first + r / a.q_heads) * a.o_token +
-                           (r % a.q_heads) * a.o_head + i % a.head_dim,
-                       0.0f);
-    }
-  }
-
-  // ---- this CTA's piece of the line of blocks
-  KvWalk<RT> w;
-  {
-    const int per = static_cast<int>((bt.n_seqs + KA_WARPS * 32 - 1) / (KA_WARPS * 32));
-    const int s0 = min(tid * per, static_cast<int>(bt.n_seqs));
-    const int s1 = min(s0 + per, static_cast<int>(bt.n_seqs));
-    int64_t mine = 0;
-    for (int s = s0; s < s1; ++s) mine += kv_seq_blocks<RT>(c, bt, a.group, s);
-    mine *= c.kv_heads;
-    int64_t scan = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += v;
-    }
-    if (lane == 31) sm_sum[warp] = scan;
-    if (tid == 0) sm_start[0] = -1;
-    __syncthreads();
-    int64_t before = scan - mine, total = 0;
-#pragma unroll
-    for (int i = 0; i < KA_WARPS; ++i) {
-      if (i < warp) before += sm_sum[i];
-      total += sm_sum[i];
-    }
-    // as many CTAs as have min_blocks each, all of the grid when the line is long
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + min_blocks - 1) / min_blocks);
-    const int64_t p0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
-    const int64_t p1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
-    if (p0 < p1 && before <= p0 && p0 < before + mine) {
-      int64_t at = before;
-      for (w.s = s0; w.s < s1 - 1; ++w.s) {
-        const int64_t n = kv_seq_blocks<RT>(c, bt, a.group, w.s) * c.kv_heads;
-        if (p0 < at + n) break;
-        at += n;
-      }
-      w.set_seq(c, bt, a.group);
-      for (w.tile = 0;; ++w.tile) {
-        w.set_tile(a.group);
-        const int64_t n = static_cast<int64_t>(w.nb) * c.kv_heads;
-        if (p0 < at + n || w.tile >= w.tiles - 1) break;
-        at += n;
-      }
-      sm_start[0] = w.s, sm_start[1] = w.tile;
-      sm_start[2] = static_cast<int>((p0 - at) / w.nb), sm_start[3] = static_cast<int>((p0 - at) % w.nb);
-    }
-    __syncthreads();
-    if (sm_start[0] < 0) {
-      if (tid == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-      return;
-    }
-    w.s = sm_start[0], w.tile = sm_start[1], w.head = sm_start[2], w.b = sm_start[3];
-    w.left = static_cast<int>(p1 - p0);
-    w.set_seq(c, bt, a.group);
-    w.set_tile(a.group);
-    w.e = min(w.nb, w.b + w.left);
+  kv_zero_rest<T>(bt, a);
+  KvWalk<RT, KV_BLOCK> w;
+  if (!kv_walk_start<KA_WARPS * 32>(w, c, bt, a, min_blocks)) {
+    if (tid == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
   }
 
   // ---- loads: a second walk, STAGES - 1 blocks of this warp ahead
   const uint32_t ring = smem_u32(smem) + warp * SH::STAGES * SH::STAGE;
-  KvWalk<RT> ld = w;
+  KvWalk<RT, KV_BLOCK> ld = w;
   int ld_blk = ld.b + warp;  // this warp's next block
   const auto ld_settle = [&] {  // moves on to the piece that holds this warp's next block
     while (ld.left > 0 && ld_blk >= ld.e) {
-      ld.next(c, bt, a.group);
+      ld.next(c, bt, a);
       ld_blk = ld.b + warp;
     }
   };
@@ -542,13 +552,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
     }
     first_piece = false;
     __syncthreads();
-    w.next(c, bt, a.group);
+    w.next(c, bt, a);
   }
   cp_async_wait<0>();
 }
 
 // Joins the partial rows of every unit that a CTA began and did not end: its own, then those of the
-// following CTAs up to the one that ended the unit.
+// following CTAs up to the one that ended the unit.  Rows are shared out along grid.y.
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBatch bt, KvAttn a, int ctas) {
   pdl_wait();
@@ -562,7 +572,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBat
   const auto slot = [&](int cta, int r) {
     return a.ws + (static_cast<int64_t>(cta * 2 + (cta == static_cast<int>(blockIdx.x))) * RT + r) * (D + 2);
   };
-  for (int i = threadIdx.x; i < rows * D; i += 256) {
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * D; i += 256 * gridDim.y) {
     const int r = i / D, d = i % D;
     float top = -1e30f;
     for (int x = blockIdx.x; x <= last; ++x) top = fmaxf(top, slot(x, r)[0]);
@@ -582,94 +592,4 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBat
   }
 }
 
-inline int kv_sm_count() {
-  int sms = 0;
-  return rt_sm_count(&sms) == RT_OK ? sms : 0;
-}
-constexpr int KA_GRID = 2;  // CTAs per SM at most
-
-template <typename T, int D, int NT>
-int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
-  using SH = KaShape<T, D, NT>;
-  auto *kernel = kv_attention_kernel<T, D, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::SMEM);
-  if (e != cudaSuccess) return fail(RT_ERR_CUDA, "kv_attention: %s", cudaGetErrorString(e));
-  const int ctas = sms * SH::MIN_CTAS;
-  launch_k(kernel, ctas, KA_WARPS * 32, SH::SMEM, s, c, bt, a, KA_WARPS);
-  launch_k(kv_attention_join_kernel<T, D, SH::RT>, ctas, 256, 0, s, c, bt, a, ctas);
-  return check_launch("kv_attention");
-}
-template <typename T>
-int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
-  // 16-row tiles once the sequences average more than 8 rows per kv head
-  const bool wide = bt.n_tokens * a.group > 8 * bt.n_seqs;
-  switch (c.dim) {
-    case 32:
-      return wide ? kv_attention_run<T, 32, 2>(c, bt, a, sms, s) : kv_attention_run<T, 32, 1>(c, bt, a, sms, s);
-    case 64:
-      return wide ? kv_attention_run<T, 64, 2>(c, bt, a, sms, s) : kv_attention_run<T, 64, 1>(c, bt, a, sms, s);
-    case 128:
-      return wide ? kv_attention_run<T, 128, 2>(c, bt, a, sms, s) : kv_attention_run<T, 128, 1>(c, bt, a, sms, s);
-    default:
-      return kv_attention_run<T, 256, 1>(c, bt, a, sms, s);
-  }
-}
-
 }  // namespace rt
-
-using namespace rt;
-
-extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
-                                                   int64_t kv_heads, int64_t padded_dim) {
-  (void)n_seqs, (void)n_tokens, (void)q_heads, (void)kv_heads;
-  const int64_t ctas = static_cast<int64_t>(kv_sm_count()) * KA_GRID;
-  return ctas * 16 + ctas * 2 * 16 * (padded_dim + 2) * 4;
-}
-
-extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
-                               int64_t q_stride_head, int64_t q_heads, int64_t head_dim,
-                               const void *codes, const float *scales, int64_t n_pages,
-                               int64_t kv_heads, int64_t page_size, int64_t padded_dim,
-                               const int32_t *page_table, int64_t pages_per_seq,
-                               const int32_t *kv_lens, const int32_t *cu_tokens, int64_t n_seqs,
-                               int64_t n_tokens, double softmax_scale, void *out,
-                               int64_t o_stride_token, int64_t o_stride_head, void *workspace,
-                               int64_t workspace_bytes, void *stream) {
-  KvCache c;
-  KvBatch b;
-  if (int rc = kv_check("kv_attention", codes, scales, n_pages, kv_heads, page_size, padded_dim,
-                        head_dim, &c))
-    return rc;
-  if (int rc = kv_check_batch("kv_attention", page_table, pages_per_seq, kv_lens, cu_tokens, n_seqs,
-                              n_tokens, page_size, &b))
-    return rc;
-  if (dtype != RT_F32 && dtype != RT_BF16)
-    return fail(RT_ERR_DTYPE, "kv_attention: queries must be float32 or bfloat16");
-  if (q_heads <= 0 || q_heads % kv_heads != 0)
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: query heads must be a multiple of kv heads");
-  if (!(softmax_scale - softmax_scale == 0))
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: softmax scale must be finite");
-  if (n_tokens == 0) return RT_OK;
-  if (q == nullptr || out == nullptr)
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: null pointer");
-  if (n_tokens * q_heads > INT32_MAX - 64) return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
-  const int sms = kv_sm_count();
-  if (sms <= 0) return fail(RT_ERR_CUDA, "kv_attention: no device");
-  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-      workspace_bytes < rt_kv_attention_workspace_bytes(n_seqs, n_tokens, q_heads, kv_heads, padded_dim))
-    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: workspace too small or not 256-byte aligned");
-  KvAttn a{};
-  a.q = q, a.q_token = q_stride_token, a.q_head = q_stride_head;
-  a.out = out, a.o_token = o_stride_token, a.o_head = o_stride_head;
-  a.q_heads = static_cast<int>(q_heads), a.group = static_cast<int>(q_heads / kv_heads);
-  a.head_dim = static_cast<int>(head_dim);
-  a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
-  const int es = dtype == RT_F32 ? 4 : 2;
-  a.q_vec = head_dim == padded_dim && aligned16(q) && (q_stride_token * es) % 16 == 0 &&
-            (q_stride_head * es) % 16 == 0;
-  const int64_t ctas = static_cast<int64_t>(sms) * KA_GRID;
-  a.meta = static_cast<int4 *>(workspace);
-  a.ws = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + ctas * 16);
-  return dtype == RT_F32 ? kv_attention_width<float>(c, b, a, sms, as_stream(stream))
-                         : kv_attention_width<__nv_bfloat16>(c, b, a, sms, as_stream(stream));
-}

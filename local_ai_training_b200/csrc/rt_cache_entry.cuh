@@ -1,0 +1,155 @@
+// rt_cache_entry.cuh — the attention entry point: which kernels a batch takes, their grids and workspace.
+#pragma once
+
+#include "rt_cache_prefill.cuh"
+
+namespace rt {
+
+inline int kv_sm_count() {
+  int sms = 0;
+  return rt_sm_count(&sms) == RT_OK ? sms : 0;
+}
+constexpr int KA_GRID = 2;       // CTAs per SM of the few-row kernel, at most
+constexpr int KP_MIN_ROWS = 64;  // rows per kv head from which a sequence takes the tcgen05 kernel
+
+// Whether any sequence of the batch can take the tcgen05 kernel.
+inline bool kv_prefill_fits(int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+  return (dim == 64 || dim == 128) && n_tokens * (q_heads / kv_heads) >= KP_MIN_ROWS;
+}
+inline int64_t kv_few_bytes(int64_t sms, int64_t dim) {
+  return sms * KA_GRID * (16 + 2 * 16 * (dim + 2) * 4);
+}
+inline int64_t kv_prefill_bytes(int64_t sms, int64_t dim) { return sms * (16 + 2 * 256 * (dim + 2) * 4); }
+
+// cudaFuncSetAttribute once per kernel and device
+template <typename K>
+inline int kv_allow_smem(K *kernel, int bytes, std::mutex &mu, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return fail(RT_ERR_CUDA, "kv_attention: no device");
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(RT_ERR_CUDA, "kv_attention: %s", cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  return RT_OK;
+}
+
+template <typename T, int D, int NT>
+int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+  using SH = KaShape<T, D, NT>;
+  static std::mutex mu;
+  static bool done[64] = {false};
+  auto *kernel = kv_attention_kernel<T, D, NT>;
+  if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
+  const int ctas = sms * SH::MIN_CTAS;
+  launch_k(kernel, ctas, KA_WARPS * 32, SH::SMEM, s, c, bt, a, KA_WARPS);
+  launch_k(kv_attention_join_kernel<T, D, SH::RT>, ctas, 256, 0, s, c, bt, a, ctas);
+  return check_launch("kv_attention");
+}
+template <int D>
+int kv_prefill_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+  using SH = KpShape<D>;
+  static std::mutex mu;
+  static bool done[64] = {false};
+  auto *kernel = kv_prefill_kernel<D>;
+  if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
+  launch_k(kernel, sms, SH::THREADS, SH::SMEM, s, c, bt, a, 2);
+  launch_k(kv_attention_join_kernel<__nv_bfloat16, D, SH::RT>, dim3(sms, 8), 256, 0, s, c, bt, a, sms);
+  return check_launch("kv_attention");
+}
+template <typename T>
+int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+  // 16-row tiles once the sequences average more than 8 rows per kv head
+  const bool wide = bt.n_tokens * a.group > 8 * bt.n_seqs;
+  switch (c.dim) {
+    case 32:
+      return wide ? kv_attention_run<T, 32, 2>(c, bt, a, sms, s) : kv_attention_run<T, 32, 1>(c, bt, a, sms, s);
+    case 64:
+      return wide ? kv_attention_run<T, 64, 2>(c, bt, a, sms, s) : kv_attention_run<T, 64, 1>(c, bt, a, sms, s);
+    case 128:
+      return wide ? kv_attention_run<T, 128, 2>(c, bt, a, sms, s) : kv_attention_run<T, 128, 1>(c, bt, a, sms, s);
+    default:
+      return kv_attention_run<T, 256, 1>(c, bt, a, sms, s);
+  }
+}
+
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
+                                                   int64_t kv_heads, int64_t padded_dim) {
+  (void)n_seqs;
+  if (kv_heads <= 0 || n_tokens <= 0) return 0;
+  const int64_t sms = kv_sm_count();
+  return kv_few_bytes(sms, padded_dim) +
+         (kv_prefill_fits(n_tokens, q_heads, kv_heads, padded_dim) ? kv_prefill_bytes(sms, padded_dim) : 0);
+}
+
+extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
+                               int64_t q_stride_head, int64_t q_heads, int64_t head_dim,
+                               const void *codes, const float *scales, int64_t n_pages,
+                               int64_t kv_heads, int64_t page_size, int64_t padded_dim,
+                               const int32_t *page_table, int64_t pages_per_seq,
+                               const int32_t *kv_lens, const int32_t *cu_tokens, int64_t n_seqs,
+                               int64_t n_tokens, double softmax_scale, void *out,
+                               int64_t o_stride_token, int64_t o_stride_head, void *workspace,
+                               int64_t workspace_bytes, void *stream) {
+  KvCache c;
+  KvBatch b;
+  if (int rc = kv_check("kv_attention", codes, scales, n_pages, kv_heads, page_size, padded_dim,
+                        head_dim, &c))
+    return rc;
+  if (int rc = kv_check_batch("kv_attention", page_table, pages_per_seq, kv_lens, cu_tokens, n_seqs,
+                              n_tokens, page_size, &b))
+    return rc;
+  if (dtype != RT_F32 && dtype != RT_BF16)
+    return fail(RT_ERR_DTYPE, "kv_attention: queries must be float32 or bfloat16");
+  if (q_heads <= 0 || q_heads % kv_heads != 0)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: query heads must be a multiple of kv heads");
+  if (!(softmax_scale - softmax_scale == 0))
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: softmax scale must be finite");
+  if (n_tokens == 0) return RT_OK;
+  if (q == nullptr || out == nullptr)
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: null pointer");
+  if (n_tokens * q_heads > INT32_MAX - 64) return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
+  const int sms = kv_sm_count();
+  if (sms <= 0) return fail(RT_ERR_CUDA, "kv_attention: no device");
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+      workspace_bytes < rt_kv_attention_workspace_bytes(n_seqs, n_tokens, q_heads, kv_heads, padded_dim))
+    return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: workspace too small or not 256-byte aligned");
+  KvAttn a{};
+  a.q = q, a.q_token = q_stride_token, a.q_head = q_stride_head;
+  a.out = out, a.o_token = o_stride_token, a.o_head = o_stride_head;
+  a.q_heads = static_cast<int>(q_heads), a.group = static_cast<int>(q_heads / kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  const int es = dtype == RT_F32 ? 4 : 2;
+  const auto vec = [&](const void *p, int64_t token, int64_t head) {
+    return head_dim == padded_dim && aligned16(p) && token * es % 16 == 0 && head * es % 16 == 0;
+  };
+  a.q_vec = vec(q, q_stride_token, q_stride_head);
+  a.o_vec = vec(out, o_stride_token, o_stride_head);
+  a.rows_lo = 0, a.rows_hi = INT32_MAX;
+  // Rows are known on the device only: a batch that may hold sequences of both kinds launches both
+  // kernels, and each takes its own sequences.  One sequence is a prompt piece when it is long enough.
+  const bool prefill = dtype == RT_BF16 && kv_prefill_fits(n_tokens, q_heads, kv_heads, padded_dim);
+  cudaStream_t s = as_stream(stream);
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  if (prefill) {
+    KvAttn p = a;
+    if (n_seqs > 1) p.rows_lo = a.rows_hi = KP_MIN_ROWS;
+    uint8_t *at = ws + kv_few_bytes(sms, padded_dim);
+    p.meta = reinterpret_cast<int4 *>(at);
+    p.ws = reinterpret_cast<float *>(at + sms * 16);
+    if (int rc = padded_dim == 64 ? kv_prefill_run<64>(c, b, p, sms, s) : kv_prefill_run<128>(c, b, p, sms, s))
+      return rc;
+    if (n_seqs <= 1) return RT_OK;
+  }
+  a.meta = reinterpret_cast<int4 *>(ws);
+  a.ws = reinterpret_cast<float *>(ws + sms * KA_GRID * 16);
+  return dtype == RT_F32 ? kv_attention_width<float>(c, b, a, sms, s)
+                         : kv_attention_width<__nv_bfloat16>(c, b, a, sms, s);
+}
