@@ -59,14 +59,20 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatch &b, int page_size, int64_t
     raise_status(RT_STATUS_INDEX_RANGE);
   return q;
 }
+// The table's entry for block `blk` of sequence s, of whose `len` tokens the block holds some; no page
+// (-1) for a block behind them.  kv_page_ok: whether it names a page; what does not is flagged.
+__device__ __forceinline__ int32_t kv_entry(const KvCache &c, const KvBatch &b, int64_t s, int blk, int len) {
+  return blk * KV_BLOCK < len ? __ldg(b.page_table + s * b.pages_per_seq + (blk >> (c.page_shift - 4))) : -1;
+}
+__device__ __forceinline__ bool kv_page_ok(const KvCache &c, int32_t p, int blk, int len) {
+  const bool ok = p >= 0 && p < c.n_pages;
+  if (!ok && blk * KV_BLOCK < len) raise_status(RT_STATUS_INDEX_RANGE);
+  return ok;
+}
 // Page that holds block `blk` of sequence s, or -1 (flagged) when the table names none.
 __device__ __forceinline__ int64_t kv_page(const KvCache &c, const KvBatch &b, int64_t s, int blk) {
-  const int32_t p = __ldg(b.page_table + s * b.pages_per_seq + (blk >> (c.page_shift - 4)));
-  if (p < 0 || p >= c.n_pages) {
-    raise_status(RT_STATUS_INDEX_RANGE);
-    return -1;
-  }
-  return p;
+  const int32_t p = kv_entry(c, b, s, blk, INT32_MAX);
+  return kv_page_ok(c, p, blk, INT32_MAX) ? p : -1;
 }
 // The sequence whose rows hold row t (cu[s] <= t < cu[s + 1]), or -1.
 __device__ __forceinline__ int64_t kv_seq_of(const int32_t *cu, int64_t n_seqs, int64_t t) {

@@ -93,10 +93,20 @@ struct KvAttn {
   int q_heads, group, head_dim;
   float scale_log2;  // softmax scale · log2(e)
   bool q_vec, o_vec;  // rows of q / out allow 16-byte accesses over the whole stored width
+  int group_shift;      // log2(group), or -1
   int rows_lo, rows_hi;  // this launch takes the sequences with rows_lo <= rows per kv head < rows_hi
-  float *ws;         // partial rows: [2 · grid][RT][D + 2]
+  float *ws;         // partial rows: [2 · grid][RT][4 + D], m and l first
   int4 *meta;        // per CTA: {sequence or -1, row tile, kv head, head slot ends its unit}
 };
+
+// Token and head within the group of a sequence's row (rows are token-major).
+__device__ __forceinline__ void kv_row(const KvAttn &a, int row, int &token, int &sub) {
+  if (a.group_shift >= 0) {
+    token = row >> a.group_shift, sub = row & (a.group - 1);
+  } else {
+    token = row / a.group, sub = row % a.group;
+  }
+}
 
 // Walks the line of (sequence, row tile, kv head) units from a CTA's first block on.  A unit is RT
 // query rows (token-major, the group's heads innermost) and the blocks of KEYS keys that they see.
@@ -270,20 +280,22 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
   const uint32_t ring = smem_u32(smem) + warp * SH::STAGES * SH::STAGE;
   KvWalk<RT, KV_BLOCK> ld = w;
   int ld_blk = ld.b + warp;  // this warp's next block
+  int32_t ld_page;  // its table entry, looked up a step before it is used
   const auto ld_settle = [&] {  // moves on to the piece that holds this warp's next block
     while (ld.left > 0 && ld_blk >= ld.e) {
       ld.next(c, bt, a);
       ld_blk = ld.b + warp;
     }
+    ld_page = ld.left > 0 ? kv_entry(c, bt, ld.s, ld_blk, ld.q.len) : -1;
   };
+  ld_settle();
   const int koff = g * D + t4 * SH::KB;
   const int voff = (D >= 128 ? g * 16 : g * SH::VB) + 2 * t4 * D;
   const int64_t part = static_cast<int64_t>(c.kv_heads) * c.page_size * D;
   const auto fetch = [&](int stage) {
-    ld_settle();
     if (ld.left > 0) {
       const uint32_t st = ring + stage * SH::STAGE;
-      const int64_t page = ld_blk * KV_BLOCK < ld.q.len ? kv_page(c, bt, ld.s, ld_blk) : -1;
+      const int64_t page = kv_page_ok(c, ld_page, ld_blk, ld.q.len) ? ld_page : -1;
       const int in_page = ld_blk & ((c.page_size >> 4) - 1);
       if (page >= 0) {
         const int8_t *kp = c.block(page, 0, ld.head, in_page);
@@ -307,6 +319,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
       if (lane == 2)
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(st + 32 * D + 8), "r"(page >= 0 ? 1 : 0) : "memory");
       ld_blk += KA_WARPS;
+      ld_settle();
     }
     cp_async_commit();
   };
@@ -539,8 +552,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
                            den > 0.0f ? __fdividef(sum, den) : 0.0f);
         }
       } else {
-        float *dst = a.ws + (static_cast<int64_t>(slot) * RT + r) * (D + 2);
-        dst[2 + d] = sum;
+        float *dst = a.ws + (static_cast<int64_t>(slot) * RT + r) * (D + 4);
+        dst[4 + d] = sum;
         if (d == 0) dst[0] = top, dst[1] = den;
       }
     }
@@ -558,37 +571,72 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
 }
 
 // Joins the partial rows of every unit that a CTA began and did not end: its own, then those of the
-// following CTAs up to the one that ended the unit.  Rows are shared out along grid.y.
+// following CTAs up to the one that ended the unit, in that order.  One warp per row, eight rows per
+// CTA (grid.y covers a unit's rows); lanes over the partials for the factors, then over the width.
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBatch bt, KvAttn a, int ctas) {
+  constexpr int W = D >= 128 ? 4 : D / 32, CH = D / (32 * W);  // floats of a lane's access, accesses
   pdl_wait();
   pdl_trigger();
   const int4 mt = a.meta[blockIdx.x];
   if (mt.x < 0) return;
-  int last = blockIdx.x + 1;
-  while (last < ctas - 1 && a.meta[last].w == 0) ++last;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
   const KvSeq q = kv_seq(bt, c.page_size, mt.x);
-  const int row0 = mt.y * RT, rows = min(RT, q.n * a.group - row0);
-  const auto slot = [&](int cta, int r) {
-    return a.ws + (static_cast<int64_t>(cta * 2 + (cta == static_cast<int>(blockIdx.x))) * RT + r) * (D + 2);
+  const int row = mt.y * RT + r;
+  if (row >= q.n * a.group) return;
+  int last = blockIdx.x + 1;  // the CTA that ended the unit
+  for (;; last += 32) {
+    const int x = last + lane;
+    const uint32_t ends = __ballot_sync(0xffffffffu, x >= ctas - 1 || a.meta[x].w != 0);
+    if (ends != 0) {
+      last = min(last + __ffs(ends) - 1, ctas - 1);
+      break;
+    }
+  }
+  const auto slot = [&](int cta) {
+    return a.ws + (static_cast<int64_t>(cta * 2 + (cta == static_cast<int>(blockIdx.x))) * RT + r) * (D + 4);
   };
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * D; i += 256 * gridDim.y) {
-    const int r = i / D, d = i % D;
-    float top = -1e30f;
-    for (int x = blockIdx.x; x <= last; ++x) top = fmaxf(top, slot(x, r)[0]);
-    float sum = 0.0f, den = 0.0f;
-    for (int x = blockIdx.x; x <= last; ++x) {
-      const float *p = slot(x, r);
-      const float f = ex2(p[0] - top);
-      den += f * p[1];
-      sum += f * p[2 + d];
+  const int first = blockIdx.x;
+  float top = -1e30f;
+  for (int x = first + lane; x <= last; x += 32) top = fmaxf(top, slot(x)[0]);
+  top = warp_max(top);
+  float den = 0.0f, acc[CH * W];
+#pragma unroll
+  for (int i = 0; i < CH * W; ++i) acc[i] = 0.0f;
+  for (int x0 = first; x0 <= last; x0 += 32) {
+    float f = 0.0f;
+    if (x0 + lane <= last) {
+      const float2 ml = *reinterpret_cast<const float2 *>(slot(x0 + lane));
+      f = ex2(ml.x - top);
+      den += f * ml.y;
     }
-    if (d < a.head_dim) {
-      const int tok = (row0 + r) / a.group, h = mt.z * a.group + (row0 + r) % a.group;
-      store_from_float(static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(tok)) * a.o_token +
-                           static_cast<int64_t>(h) * a.o_head + d,
-                       den > 0.0f ? __fdividef(sum, den) : 0.0f);
+    const int n = min(32, last + 1 - x0);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float g = __shfl_sync(0xffffffffu, f, i);
+      const float *p = slot(x0 + i) + 4 + lane * W;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        float v[W];
+        if constexpr (W == 4)
+          *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p + k * 128);
+        else if constexpr (W == 2)
+          *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
+        else
+          v[0] = *p;
+#pragma unroll
+        for (int j = 0; j < W; ++j) acc[k * W + j] += g * v[j];
+      }
     }
+  }
+  den = warp_sum_butterfly(den);
+  const float inv = den > 0.0f ? __fdividef(1.0f, den) : 0.0f;
+  T *o = static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(row / a.group)) * a.o_token +
+         static_cast<int64_t>(mt.z * a.group + row % a.group) * a.o_head;
+#pragma unroll
+  for (int i = 0; i < CH * W; ++i) {
+    const int d = (i / W) * 128 + lane * W + i % W;
+    if (d < a.head_dim) store_from_float(o + d, acc[i] * inv);
   }
 }
 

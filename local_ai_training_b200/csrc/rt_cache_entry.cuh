@@ -17,9 +17,9 @@ inline bool kv_prefill_fits(int64_t n_tokens, int64_t q_heads, int64_t kv_heads,
   return (dim == 64 || dim == 128) && n_tokens * (q_heads / kv_heads) >= KP_MIN_ROWS;
 }
 inline int64_t kv_few_bytes(int64_t sms, int64_t dim) {
-  return sms * KA_GRID * (16 + 2 * 16 * (dim + 2) * 4);
+  return sms * KA_GRID * (16 + 2 * 16 * (dim + 4) * 4);
 }
-inline int64_t kv_prefill_bytes(int64_t sms, int64_t dim) { return sms * (16 + 2 * 256 * (dim + 2) * 4); }
+inline int64_t kv_prefill_bytes(int64_t sms, int64_t dim) { return sms * (16 + 2 * 256 * (dim + 4) * 4); }
 
 // cudaFuncSetAttribute once per kernel and device
 template <typename K>
@@ -45,7 +45,8 @@ int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int s
   if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
   const int ctas = sms * SH::MIN_CTAS;
   launch_k(kernel, ctas, KA_WARPS * 32, SH::SMEM, s, c, bt, a, KA_WARPS);
-  launch_k(kv_attention_join_kernel<T, D, SH::RT>, ctas, 256, 0, s, c, bt, a, ctas);
+  launch_k(kv_attention_join_kernel<T, D, SH::RT>, dim3(ctas, SH::RT / 8), 256, 0, s, c, bt,
+           a, ctas);
   return check_launch("kv_attention");
 }
 template <int D>
@@ -56,7 +57,8 @@ int kv_prefill_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms
   auto *kernel = kv_prefill_kernel<D>;
   if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
   launch_k(kernel, sms, SH::THREADS, SH::SMEM, s, c, bt, a, 2);
-  launch_k(kv_attention_join_kernel<__nv_bfloat16, D, SH::RT>, dim3(sms, 8), 256, 0, s, c, bt, a, sms);
+  launch_k(kv_attention_join_kernel<__nv_bfloat16, D, SH::RT>, dim3(sms, SH::RT / 8), 256, 0, s, c, bt,
+           a, sms);
   return check_launch("kv_attention");
 }
 template <typename T>
@@ -125,6 +127,9 @@ extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
   a.out = out, a.o_token = o_stride_token, a.o_head = o_stride_head;
   a.q_heads = static_cast<int>(q_heads), a.group = static_cast<int>(q_heads / kv_heads);
   a.head_dim = static_cast<int>(head_dim);
+  a.group_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a.group == 1 << i) a.group_shift = i;
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   const int es = dtype == RT_F32 ? 4 : 2;
   const auto vec = [&](const void *p, int64_t token, int64_t head) {

@@ -9,7 +9,7 @@
 //   warps 0-3 / 4-7  softmax of row tile A / B, one row per thread (its TMEM lane): scores from tensor
 //                    memory, running maximum, weights back to tensor memory as bf16 over the scores
 //   warps 8-11       codes from the pages -> bf16 (exact) -> shared memory in the 128-byte swizzle
-//   warp 12          one thread issues S = Q K^T (both from shared memory) and O += P V (P from
+//   warp 12          (of the fourth warpgroup; the other three idle) one thread issues S = Q K^T (both from shared memory) and O += P V (P from
 //                    tensor memory); completion by tcgen05.commit
 // The block scales are folded into the scores and the weights (a factor per 16 keys).  The weight
 // 2^(t - m)·sv is rounded to bf16 (bf16 queries only; the sum of weights keeps 32 bits).  The running
@@ -49,6 +49,60 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// 16 bytes global -> shared, zeros when `in` is false.
+__device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void *gmem, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0)
+               : "memory");
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+template <int N>
+__device__ __forceinline__ void set_registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Barrier of 128 threads (one row tile's softmax warps) that also ands a flag over them.
+__device__ __forceinline__ bool warpgroup_and(int id, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -62,12 +116,15 @@ struct KpShape {
   static constexpr int STAGES = 2;
   static constexpr int SCALES = 4;               // ring of the block factors
   static constexpr int Q_OFF = 0, K_OFF = 2 * TILE, V_OFF = K_OFF + STAGES * TILE;
-  static constexpr int F_OFF = V_OFF + STAGES * TILE;
+  static constexpr int RAW_OFF = V_OFF + STAGES * TILE;  // codes of one tile, K then V
+  static constexpr int F_OFF = RAW_OFF + TILE;
   static constexpr int BAR_OFF = F_OFF + SCALES * 80;
   // one CTA per SM: each takes all 512 columns of tensor memory
   static constexpr int SMEM_USED = BAR_OFF + 256 + 1024;
   static constexpr int SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;
-  static constexpr int THREADS = 13 * 32;
+  static constexpr int THREADS = 16 * 32;
+  // registers per thread of the four warpgroups: 2 · 160 + 128 + 64 = 4 · 128, the launch's own
+  static constexpr int R_SOFTMAX = 160, R_ISSUE = 64;
   static constexpr uint32_t COL_S = 0, COL_O = 256;  // + 128 (scores) or + D (outputs) for row tile B
   static constexpr uint32_t IDESC_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((KEYS >> 3) << 17) | ((ROWS >> 4) << 24);
   static constexpr uint32_t IDESC_PV =
@@ -76,6 +133,7 @@ struct KpShape {
 struct KpBars {
   uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], f_full[4], s_full[2], p_ready[2], o_done[2];
   uint32_t tmem;
+  int piece[4];  // the piece's tiles: first, end, ends of row tiles A and B
 };
 static_assert(sizeof(KpBars) <= 256, "KpBars");
 struct KpFactors {  // one tile's block factors
@@ -135,6 +193,7 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
   };
 
   if (warp < 8) {
+    set_registers_up<SH::R_SOFTMAX>();
     // ================================================================ softmax of row tile x
     const int x = warp >> 2, r = tid & 127;  // r: row of the tile, TMEM lane
     const uint32_t t_s = tmem + SH::COL_S + x * 128 + (static_cast<uint32_t>(warp & 3) << 21);
@@ -149,30 +208,31 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
       {
         constexpr int CH = D / 8;  // 16-byte chunks of a row
         uint8_t *qt = smem + SH::Q_OFF + x * SH::TILE;
-#pragma unroll 4
-        for (int i = 0; i < CH; ++i) {
-          const int id = i * 128 + r, qr = id / CH, ch = id % CH;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (qr < rows) {
-            const int row = row0 + qr;
-            const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(a.q) +
-                                      (w.q.c0 + static_cast<int64_t>(row / a.group)) * a.q_token +
-                                      static_cast<int64_t>(w.head * a.group + row % a.group) * a.q_head;
-            if (a.q_vec) {
-              v = *reinterpret_cast<const uint4 *>(qp + ch * 8);
-            } else {
-              uint32_t u[8];
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                u[k] = ch * 8 + k < a.head_dim
-                           ? *reinterpret_cast<const uint16_t *>(qp + ch * 8 + k)
-                           : 0u;
-              v = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+        const bool direct = a.q_vec && !flip;
+#pragma unroll 1
+        for (int id = r; id < CH * 128; id += 128) {
+          const int qr = id / CH, ch = id % CH;
+          const bool in = qr < rows;
+          int token, sub;
+          kv_row(a, in ? row0 + qr : 0, token, sub);
+          const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(a.q) +
+                                    (w.q.c0 + static_cast<int64_t>(token)) * a.q_token +
+                                    static_cast<int64_t>(w.head * a.group + sub) * a.q_head + ch * 8;
+          uint8_t *dst = qt + (ch >> 3) * SH::SUB + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4);
+          if (direct) {
+            cp_async16_zfill(smem_u32(dst), qp, in);
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) {
+              uint32_t u = in && ch * 8 + k < a.head_dim ? *reinterpret_cast<const uint16_t *>(qp + k) : 0u;
+              if (flip) u ^= 0x8000u;
+              *reinterpret_cast<uint16_t *>(dst + 2 * k) = static_cast<uint16_t>(u);
             }
-            if (flip) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
           }
-          *reinterpret_cast<uint4 *>(qt + (ch >> 3) * SH::SUB + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4)) = v;
         }
+        cp_async_commit();
+        cp_async_wait<0>();
+        if (tid == 0) bar->piece[0] = w.b, bar->piece[1] = w.e, bar->piece[2] = tiles_of(0), bar->piece[3] = tiles_of(1);
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(&bar->q_ready);
@@ -183,7 +243,8 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
       const int end = tiles_of(x);
       const int tok = (row0 + min(r, max(rows - 1, 0))) / a.group;
       const int lim = min(w.q.start + tok + 1, w.q.len);  // keys this row sees
-      float m = -1e30f, l = 0.0f;
+      float m = -1e30f;
+      float2 l2 = make_float2(0.0f, 0.0f);  // sum of weights, even and odd keys
       for (int j = w.b; j < end && ok; ++j) {
         const uint32_t f_at = n_f + static_cast<uint32_t>(j - w.b);
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->f_full[f_at & 3], (f_at >> 2) & 1) &&
@@ -195,37 +256,47 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
         const int seen = lim - j * SH::KEYS;  // keys of this tile the row sees
         const uint32_t blocks = f->blocks;
         const bool cut = __any_sync(0xffffffffu, seen < SH::KEYS) || blocks != 0xFFu;
-        const auto hidden = [&](int col) { return col >= seen || ((blocks >> (col >> 4)) & 1) == 0; };
+        // bit i of keep(h): key 32 h + i of the tile is seen
+        const auto keep = [&](int h) {
+          const int n = min(max(seen - h * 32, 0), 32);
+          const uint32_t in = n == 32 ? 0xFFFFFFFFu : (1u << n) - 1;
+          return in & ((blocks >> (2 * h) & 1) * 0xFFFFu | (blocks >> (2 * h + 1) & 1) * 0xFFFF0000u);
+        };
+        uint32_t s[2][32];
         // ---- the tile's maximum
         float top = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(t_s + h * 32, s);
-          tmem_ld_wait_regs(s);
+#pragma unroll 1
+        for (int h = 0; h < 4; h += 2) {
+          tmem_ld_32x32b_x32(t_s + h * 32, s[0]);
+          tmem_ld_32x32b_x32(t_s + h * 32 + 32, s[1]);
+          tmem_ld_wait_regs(s[0]);
+          tmem_regs_after_wait(s[1]);
           if (cut) {
+            const uint32_t k0 = keep(h), k1 = keep(h + 1);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (hidden(h * 32 + i)) s[i] = 0xFF800000u;  // -inf
+            for (int i = 0; i < 32; ++i) {
+              if ((k0 >> i & 1) == 0) s[0][i] = 0xFF800000u;  // -inf
+              if ((k1 >> i & 1) == 0) s[1][i] = 0xFF800000u;
+            }
           }
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            float v = __uint_as_float(s[b * 16]);
+          for (int b = 0; b < 4; ++b) {
+            float v = __uint_as_float(s[b >> 1][(b & 1) * 16]);
 #pragma unroll
-            for (int i = 1; i < 16; ++i) v = fmaxf(v, __uint_as_float(s[b * 16 + i]));
+            for (int i = 1; i < 16; ++i) v = fmaxf(v, __uint_as_float(s[b >> 1][(b & 1) * 16 + i]));
             top = fmaxf(top, v * f->k[h * 2 + b]);
           }
         }
         if (__any_sync(0xffffffffu, top > m + 8.0f)) {
           const float mn = fmaxf(m, top), g = ex2(m - mn);
           m = mn;
-          l *= g;
+          l2.x *= g, l2.y *= g;
           if (j > w.b) {
             // the products so far have been added up; the next ones wait for this tile's weights
             ok = __all_sync(0xffffffffu, mbar_wait(&bar->o_done[x], (n_o + 1) & 1));
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < D / 32; ++h) {
               uint32_t o[32];
               tmem_ld_32x32b_x32(t_o + h * 32, o);
@@ -236,80 +307,126 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
             }
           }
         }
-        // ---- weights
+        // ---- weights: a second pass over the scores (holding all 128 would spill), the next 32 under way
+        // while these are worked on
+        const auto weights = [&](int h, uint32_t (&s)[32]) {
+          float2 t[16];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t s[32], p[16];
-          tmem_ld_32x32b_x32(t_s + h * 32, s);
-          tmem_ld_wait_regs(s);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), f->k[h * 2 + (i >> 4)], -m));
-          if (cut) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (hidden(h * 32 + i)) s[i] = 0xFF800000u;
+          for (int i = 0; i < 16; ++i) {
+            const float fk = f->k[h * 2 + (i >> 3)];
+            t[i] = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
+                        make_float2(fk, fk), make_float2(-m, -m));
           }
+          if (cut) {  // (a factor of 0 would make -inf a NaN: the mask comes after it)
+            const uint32_t k = keep(h);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float p0 = ex2(__uint_as_float(s[i])), p1 = ex2(__uint_as_float(s[i + 1]));
-            const float fv = f->v[h * 2 + (i >> 4)];
-            l += p0 + p1;
-            p[i / 2] = pack_bf16x2(p0 * fv, p1 * fv);
+            for (int i = 0; i < 16; ++i) {
+              if ((k >> (2 * i) & 1) == 0) t[i].x = -INFINITY;
+              if ((k >> (2 * i + 1) & 1) == 0) t[i].y = -INFINITY;
+            }
+          }
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float fv = f->v[h * 2 + (i >> 3)];
+            const float2 e = make_float2(ex2(t[i].x), ex2(t[i].y));
+            l2 = add2(l2, e);
+            const float2 wt = mul2(e, make_float2(fv, fv));
+            p[i] = pack_bf16x2(wt.x, wt.y);
           }
           tmem_st_32x32b_x16(t_s + h * 16, p);
+        };
+        tmem_ld_32x32b_x32(t_s, s[0]);
+        tmem_ld_wait_regs(s[0]);
+#pragma unroll 1
+        for (int h = 0; h < 4; h += 2) {
+          tmem_ld_32x32b_x32(t_s + h * 32 + 32, s[1]);
+          weights(h, s[0]);
+          tmem_ld_wait_regs(s[1]);
+          if (h == 0) tmem_ld_32x32b_x32(t_s + 64, s[0]);
+          weights(h + 1, s[1]);
+          if (h == 0) tmem_ld_wait_regs(s[0]);
         }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bar->p_ready[x]);
         ++n_o;  // phases of o_done that will have completed when this tile's products are in
       }
-      // ---- the piece's rows
+      // ---- the piece's rows, through the row tile's own Q tile (its products are complete) so that
+      // global memory is written in whole rows
       const bool whole = w.b == 0 && w.e == w.nb;
       if (ok && end > w.b) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->o_done[x], (n_o + 1) & 1));
+        ok = mbar_wait(&bar->o_done[x], (n_o + 1) & 1);
         tc_fence_after();
       }
+      ok = warpgroup_and(1 + x, ok);
+      const float l = l2.x + l2.y;
       if (ok) {
         const int slot = blockIdx.x * 2 + (w.b > 0 ? 0 : 1);
-        const int row = row0 + r;
-        const float inv = l > 0.0f ? __fdividef(1.0f, l) : 0.0f;
-        float *ws = a.ws + (static_cast<int64_t>(slot) * SH::RT + x * SH::ROWS + r) * (D + 2);
-        __nv_bfloat16 *op = static_cast<__nv_bfloat16 *>(a.out) +
-                            (w.q.c0 + static_cast<int64_t>(row / a.group)) * a.o_token +
-                            static_cast<int64_t>(w.head * a.group + row % a.group) * a.o_head;
+        const float scale = !whole ? 1.0f : l > 0.0f ? __fdividef(1.0f, l) : 0.0f;
+        uint8_t *stage = smem + SH::Q_OFF + x * SH::TILE;
+        float *ws = a.ws + (static_cast<int64_t>(slot) * SH::RT + x * SH::ROWS) * (D + 4);
+        if (!whole && r < rows) *reinterpret_cast<float2 *>(ws + static_cast<int64_t>(r) * (D + 4)) = make_float2(m, l);
+        // `parts` passes of 2 D bytes a row: bf16 rows in one, fp32 rows in two
+        const int parts = whole ? 1 : 2;
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part) {
+          constexpr int PIECES = D / 8;  // 16-byte pieces of a staged row
+          const int c0 = part * (D / 2), n32 = whole ? D / 32 : D / 64;
+#pragma unroll 1
+          for (int h = 0; h < n32; ++h) {
+            uint32_t o[32];
+            if (end > w.b) {
+              tmem_ld_32x32b_x32(t_o + c0 + h * 32, o);
+              tmem_ld_wait_regs(o);
+            } else {
 #pragma unroll
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t o[32];
-          if (end > w.b) {
-            tmem_ld_32x32b_x32(t_o + h * 32, o);
-            tmem_ld_wait_regs(o);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0;
-          }
-          if (r >= rows) {
-          } else if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              *reinterpret_cast<uint2 *>(ws + 2 + h * 32 + i) = make_uint2(o[i], o[i + 1]);
-          } else if (a.o_vec) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint32_t u[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                u[k] = pack_bf16x2(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4 *>(op + h * 32 + i) = make_uint4(u[0], u[1], u[2], u[3]);
+              for (int i = 0; i < 32; ++i) o[i] = 0;
             }
-          } else {
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (h * 32 + i < a.head_dim) op[h * 32 + i] = __float2bfloat16_rn(__uint_as_float(o[i]) * inv);
+              for (int i = 0; i < 32; i += 8) {
+                uint32_t u[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  u[k] = pack_bf16x2(__uint_as_float(o[i + 2 * k]) * scale, __uint_as_float(o[i + 2 * k + 1]) * scale);
+                *reinterpret_cast<uint4 *>(stage + (r * PIECES + ((h * 4 + i / 8) ^ (r & 7))) * 16) =
+                    make_uint4(u[0], u[1], u[2], u[3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4 *>(stage + (r * PIECES + ((h * 8 + i / 4) ^ (r & 7))) * 16) =
+                    make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
           }
-          __syncwarp();
+          warpgroup_and(1 + x, true);
+#pragma unroll 1
+          for (int id = r; id < PIECES * 128; id += 128) {
+            const int sr = id / PIECES, pc = id % PIECES;
+            const uint4 v = *reinterpret_cast<const uint4 *>(stage + (sr * PIECES + (pc ^ (sr & 7))) * 16);
+            if (!whole) {
+              if (sr < rows)
+                *reinterpret_cast<uint4 *>(ws + static_cast<int64_t>(sr) * (D + 4) + 4 + c0 + pc * 4) = v;
+              continue;
+            }
+            int token, sub;
+            kv_row(a, row0 + sr, token, sub);
+            __nv_bfloat16 *op = static_cast<__nv_bfloat16 *>(a.out) +
+                                (w.q.c0 + static_cast<int64_t>(token)) * a.o_token +
+                                static_cast<int64_t>(w.head * a.group + sub) * a.o_head;
+            if (a.o_vec) {
+              if (sr < rows) *reinterpret_cast<uint4 *>(op + pc * 8) = v;
+            } else {
+              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (sr < rows && pc * 8 + k < a.head_dim)
+                  *reinterpret_cast<uint16_t *>(op + pc * 8 + k) = static_cast<uint16_t>(u[k >> 1] >> (k & 1) * 16);
+            }
+          }
+          warpgroup_and(1 + x, true);
         }
-        if (!whole && r < rows) ws[0] = m, ws[1] = l;
         tc_fence_before();
       }
       if (tid == 0) {
@@ -333,43 +450,48 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
     const float fscale = fabsf(a.scale_log2);
     uint32_t n = 0;
     bool ok = true;
-    const int64_t part = static_cast<int64_t>(c.kv_heads) * c.page_size * D;
     Walk ld = w;     // the tile whose codes are fetched next
     int ld_j = ld.b;
-    uint4 raw[2][N];
-    float fk = 0.0f, fv = 0.0f;  // thread t < 8: factors of block t
+    const auto entry = [&] {  // lane i % 8: the table's entry for the tile's block i
+      return ld.left > 0 ? kv_entry(c, bt, ld.s, ld_j * 8 + (lane & 7), ld.q.len) : -1;
+    };
+    int32_t ld_page = entry();  // looked up a tile before it is used
+    float fk = 0.0f, fv = 0.0f;  // lane i < 8: factors of block i
     bool has = false;
-    const auto fetch = [&] {
+    // The codes of the next tile come into each thread's own slots (no barrier), K and V a group each.
+    uint8_t *raw = smem + SH::RAW_OFF + t * 16;
+    const auto fetch = [&](int which) {
       if (ld.left <= 0) return;
-#pragma unroll
+      const bool ok_page = kv_page_ok(c, ld_page, ld_j * 8 + (lane & 7), ld.q.len);
+      const int32_t page = ok_page ? ld_page : 0;  // (the mask hides a block without a page)
+#pragma unroll 2
       for (int i = 0; i < N; ++i) {
-        const int row = i * RPI + prow, blk = ld_j * 8 + (row >> 4);
-        raw[0][i] = raw[1][i] = make_uint4(0, 0, 0, 0);
-        const int64_t page = blk * KV_BLOCK < ld.q.len ? kv_page(c, bt, ld.s, blk) : -1;
-        if (page >= 0) {
-          const int8_t *kp = c.block(page, 0, ld.head, blk & ((c.page_size >> 4) - 1)) + (row & 15) * D + pcol * 16;
-          raw[0][i] = *reinterpret_cast<const uint4 *>(kp);
-          raw[1][i] = *reinterpret_cast<const uint4 *>(kp + part);
-        }
+        const int row = i * RPI + prow;
+        const int8_t *p = c.block(__shfl_sync(0xffffffffu, page, row >> 4), which, ld.head,
+                                  (ld_j * 8 + (row >> 4)) & ((c.page_size >> 4) - 1)) + (row & 15) * D + pcol * 16;
+        cp_async16(raw + (which * N + i) * 2048, p);
       }
+      if (which == 0) return;
+      has = ok_page;
       if (t < 8) {
-        const int blk = ld_j * 8 + t;
-        const int64_t page = blk * KV_BLOCK < ld.q.len ? kv_page(c, bt, ld.s, blk) : -1;
-        has = page >= 0;
-        fk = has ? *c.scale(page, 0, ld.head, blk & ((c.page_size >> 4) - 1)) * fscale : 0.0f;
-        fv = has ? *c.scale(page, 1, ld.head, blk & ((c.page_size >> 4) - 1)) : 0.0f;
+        const int blk = (ld_j * 8 + t) & ((c.page_size >> 4) - 1);
+        fk = has ? *c.scale(page, 0, ld.head, blk) * fscale : 0.0f;
+        fv = has ? *c.scale(page, 1, ld.head, blk) : 0.0f;
       }
       if (++ld_j >= ld.e) {
         ld.next(c, bt, a);
         ld_j = ld.b;
       }
+      ld_page = entry();
     };
-    const auto put = [&](uint8_t *tile, const uint4 (&v)[N]) {
-#pragma unroll
+    const auto put = [&](uint8_t *tile, int which) {
+      cp_async_wait<1>();
+#pragma unroll 2
       for (int i = 0; i < N; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(raw + (which * N + i) * 2048);
         const int row = i * RPI + prow;
-        const uint2 b0 = bf16x4_of_bytes(v[i].x), b1 = bf16x4_of_bytes(v[i].y);
-        const uint2 b2 = bf16x4_of_bytes(v[i].z), b3 = bf16x4_of_bytes(v[i].w);
+        const uint2 b0 = bf16x4_of_bytes(v.x), b1 = bf16x4_of_bytes(v.y);
+        const uint2 b2 = bf16x4_of_bytes(v.z), b3 = bf16x4_of_bytes(v.w);
         uint8_t *at = tile + (pcol >> 2) * SH::SUB + row * 128;
         const int ch = (pcol & 3) * 2;
         const uint4 lo = make_uint4(b0.x, b0.y, b1.x, b1.y), hi = make_uint4(b2.x, b2.y, b3.x, b3.y);
@@ -378,91 +500,98 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
         *reinterpret_cast<uint4 *>(at + (((ch + sw) ^ (row & 7)) << 4)) = sw ? hi : lo;
         *reinterpret_cast<uint4 *>(at + (((ch + 1 - sw) ^ (row & 7)) << 4)) = sw ? lo : hi;
       }
+      fence_proxy_async_smem();
     };
-    fetch();
-    while (w.left > 0 && ok) {
-      for (int j = w.b; j < w.e; ++j, ++n) {
-        const int st = n & 1;
-        const uint32_t free_parity = ((n >> 1) & 1) ^ 1;  // a fresh barrier passes for its first use
-        if (warp == 8) {
-          KpFactors *f = reinterpret_cast<KpFactors *>(smem + SH::F_OFF + (n & 3) * 80);
-          // the slot's last readers are past: tile n - 2's scores, complete here, were issued after the
-          // softmax of tile n - 3, and the slot held tile n - 4
-          ok = __all_sync(0xffffffffu, mbar_wait(&bar->k_empty[st], free_parity));
-          const uint32_t blocks = __ballot_sync(0xffffffffu, has) & 0xFFu;
-          if (lane < 8) f->k[lane] = fk, f->v[lane] = fv;
-          if (lane == 0) f->blocks = blocks;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar->f_full[n & 3]);
-        } else if (!mbar_wait(&bar->k_empty[st], free_parity)) {
-          ok = false;
-        }
-        if (!ok) break;
-        put(smem + SH::K_OFF + st * SH::TILE, raw[0]);
-        fence_proxy_async_smem();
-        mbar_arrive(&bar->k_full[st]);
-        if (!mbar_wait(&bar->v_empty[st], free_parity)) {
-          ok = false;
-          break;
-        }
-        put(smem + SH::V_OFF + st * SH::TILE, raw[1]);
-        fence_proxy_async_smem();
-        mbar_arrive(&bar->v_full[st]);
-        fetch();
+    const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
+    // A tile's K is fetched while V of the tile before is converted: fetch(0) of the next tile needs that
+    // tile's entries, which fetch(1) of this one looked up
+    fetch(0);
+    cp_async_commit();
+    fetch(1);
+    cp_async_commit();
+    for (; n < total; ++n) {
+      const int st = n & 1;
+      // a fresh barrier passes for its first use
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar->k_empty[st], ((n >> 1) & 1) ^ 1));
+      if (!ok) break;
+      if (warp == 8) {
+        // the slot's last readers are past: tile n - 2's scores, complete here, were issued after the
+        // softmax of tile n - 3, and the slot held tile n - 4
+        KpFactors *f = reinterpret_cast<KpFactors *>(smem + SH::F_OFF + (n & 3) * 80);
+        const uint32_t blocks = __ballot_sync(0xffffffffu, has) & 0xFFu;
+        if (lane < 8) f->k[lane] = fk, f->v[lane] = fv;
+        if (lane == 0) f->blocks = blocks;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->f_full[n & 3]);
       }
-      w.next(c, bt, a);
+      put(smem + SH::K_OFF + st * SH::TILE, 0);
+      mbar_arrive(&bar->k_full[st]);
+      fetch(0);
+      cp_async_commit();
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar->v_empty[st], ((n >> 1) & 1) ^ 1));
+      if (!ok) break;
+      put(smem + SH::V_OFF + st * SH::TILE, 1);
+      mbar_arrive(&bar->v_full[st]);
+      fetch(1);
+      cp_async_commit();
     }
+    cp_async_wait<0>();
   } else {
-    if (lane == 0) {
+    set_registers_down<SH::R_ISSUE>();
+    if (warp == 12 && lane == 0) {
     // ================================================================ MMA issue
     const uint32_t q0 = smem_u32(smem + SH::Q_OFF), k0 = smem_u32(smem + SH::K_OFF), v0 = smem_u32(smem + SH::V_OFF);
     uint32_t n = 0, n_q = 0, n_p[2] = {0, 0};
     bool ok = true;
     const auto qk = [&](int x, uint32_t tile) {
       tc_fence_after();
-      const uint32_t qa = q0 + x * SH::TILE, ka = k0 + (tile & 1) * SH::TILE;
+      // (descriptor addresses count 16 bytes)
+      const uint64_t qd = make_sw128_desc(q0 + x * SH::TILE, 16, 1024);
+      const uint64_t kd = make_sw128_desc(k0 + (tile & 1) * SH::TILE, 16, 1024);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        umma_f16(tmem + SH::COL_S + x * 128, make_sw128_desc(qa + (i >> 2) * SH::SUB + (i & 3) * 32, 16, 1024),
-                 make_sw128_desc(ka + (i >> 2) * SH::SUB + (i & 3) * 32, 16, 1024), SH::IDESC_QK, i > 0);
+      for (int i = 0; i < D / 16; ++i) {
+        const uint64_t step = ((i >> 2) * SH::SUB + (i & 3) * 32) >> 4;
+        umma_f16(tmem + SH::COL_S + x * 128, qd + step, kd + step, SH::IDESC_QK, i > 0);
+      }
       umma_commit(&bar->s_full[x]);
     };
     const auto pv = [&](int x, uint32_t tile, bool fresh) {
       tc_fence_after();
-      const uint32_t va = v0 + (tile & 1) * SH::TILE;
+      const uint64_t vd = make_sw128_desc(v0 + (tile & 1) * SH::TILE, SH::SUB, 1024);
 #pragma unroll
       for (int i = 0; i < SH::KEYS / 16; ++i)
         umma_f16_ts(tmem + SH::COL_O + x * D, tmem + SH::COL_S + x * 128 + i * 8,
-                    make_sw128_desc(va + i * 2048, SH::SUB, 1024), SH::IDESC_PV, !fresh || i > 0);
+                    vd + i * (2048 >> 4), SH::IDESC_PV, !fresh || i > 0);
       umma_commit(&bar->o_done[x]);
     };
-    while (w.left > 0 && ok) {
-      const int end[2] = {tiles_of(0), tiles_of(1)};
+    const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
+    while (n < total && ok) {
       ok = mbar_wait(&bar->q_ready, n_q & 1) && mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1);
       ++n_q;
       if (!ok) break;
+      const int b = bar->piece[0], e = bar->piece[1], end[2] = {bar->piece[2], bar->piece[3]};
+#pragma unroll
       for (int x = 0; x < 2; ++x)
-        if (end[x] > w.b) qk(x, n);
+        if (end[x] > b) qk(x, n);
       umma_commit(&bar->k_empty[n & 1]);
-      for (int j = w.b; j < w.e && ok; ++j, ++n) {
+      for (int j = b; j < e && ok; ++j, ++n) {
         ok = mbar_wait(&bar->v_full[n & 1], (n >> 1) & 1);
-        const bool more = j + 1 < w.e;
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (j < end[x]) {
+        const bool more = j + 1 < e;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (ok && j < end[x]) {
             ok = mbar_wait(&bar->p_ready[x], n_p[x] & 1);
             ++n_p[x];
-            if (!ok) break;
-            pv(x, n, j == w.b);
+            if (ok) pv(x, n, j == b);
           }
           if (x == 1) umma_commit(&bar->v_empty[n & 1]);
-          if (more && j + 1 < end[x]) {
+          if (ok && more && j + 1 < end[x]) {
             ok = mbar_wait(&bar->k_full[(n + 1) & 1], ((n + 1) >> 1) & 1);
             if (ok) qk(x, n + 1);
           }
         }
         if (more && ok) umma_commit(&bar->k_empty[(n + 1) & 1]);
       }
-      if (ok) w.next(c, bt, a);
     }
     }
     __syncwarp();
