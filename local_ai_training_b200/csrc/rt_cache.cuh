@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvCopy a, int copy_blocks)
 inline int kv_check(const char *what, const void *codes, const void *scales, int64_t n_pages,
                     int64_t kv_heads, int64_t page_size, int64_t dim, int64_t head_dim,
                     KvCache *c) {
-  if (n_pages <= 0 || kv_heads <= 0 || n_pages > INT32_MAX || kv_heads > 65535)
+  if (n_pages <= 0 || kv_heads <= 0 || n_pages > INT32_MAX || kv_heads > 4096)
     return fail(RT_ERR_INVALID_ARGUMENT, "%s: cache shape", what);
   if (page_size < KV_BLOCK || page_size > 256 || (page_size & (page_size - 1)) != 0)
     return fail(RT_ERR_INVALID_ARGUMENT, "%s: page_size must be 16, 32, 64, 128 or 256", what);

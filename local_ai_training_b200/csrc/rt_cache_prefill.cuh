@@ -8,9 +8,10 @@
 // are in its softmax warps, the other's products run.
 //   warps 0-3 / 4-7  softmax of row tile A / B, one row per thread (its TMEM lane): scores from tensor
 //                    memory, running maximum, weights back to tensor memory as bf16 over the scores
-//   warps 8-11       codes from the pages -> bf16 (exact) -> shared memory in the 128-byte swizzle
-//   warp 12          (of the fourth warpgroup; the other three idle) one thread issues S = Q K^T (both from shared memory) and O += P V (P from
-//                    tensor memory); completion by tcgen05.commit
+//   warps 8-11, 12-14  K and V: codes from the pages -> bf16 (exact) -> shared memory in the 128-byte
+//                    swizzle
+//   warp 15          one thread issues S = Q K^T (both from shared memory) and O += P V (P from tensor
+//                    memory); completion by tcgen05.commit
 // The block scales are folded into the scores and the weights (a factor per 16 keys).  The weight
 // 2^(t - m)·sv is rounded to bf16 (bf16 queries only; the sum of weights keeps 32 bits).  The running
 // maximum moves, and O is rescaled, only when a score exceeds it by 2^8.
@@ -38,15 +39,16 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+// 16 columns, loaded and waited for.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 // 16 bytes global -> shared, zeros when `in` is false.
@@ -123,8 +125,8 @@ struct KpShape {
   static constexpr int SMEM_USED = BAR_OFF + 256 + 1024;
   static constexpr int SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;
   static constexpr int THREADS = 16 * 32;
-  // registers per thread of the four warpgroups: 2 · 160 + 128 + 64 = 4 · 128, the launch's own
-  static constexpr int R_SOFTMAX = 160, R_ISSUE = 64;
+  // registers per thread of the four warpgroups: 2 · 152 + 128 + 80 = 4 · 128, the launch's own
+  static constexpr int R_SOFTMAX = 152, R_REST = 80;
   static constexpr uint32_t COL_S = 0, COL_O = 256;  // + 128 (scores) or + D (outputs) for row tile B
   static constexpr uint32_t IDESC_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((KEYS >> 3) << 17) | ((ROWS >> 4) << 24);
   static constexpr uint32_t IDESC_PV =
@@ -146,6 +148,94 @@ __device__ __forceinline__ uint2 bf16x4_of_bytes(uint32_t w) {
   return make_uint2(bf16x2_of_bytes<false>(w), bf16x2_of_bytes<true>(w));
 }
 
+// Codes -> bf16 tiles: K (part 0, 128 threads) or V (part 1, 96 threads).  Thread t takes the 16-byte pieces t, t + N, ... of a
+// tile's codes, which come a tile ahead into its own slots (no barrier).  Lane i % 8 looks up block i's
+// page, a tile before it is used.
+template <int D, int part, int N>
+__device__ __forceinline__ void kv_prefill_codes(const KvCache &c, const KvBatch &bt, const KvAttn &a,
+                                                 const KvWalk<KpShape<D>::RT, KpShape<D>::KEYS> &w, uint8_t *smem,
+                                                 KpBars *bar, int t) {
+  using SH = KpShape<D>;
+  const int lane = threadIdx.x & 31;
+  constexpr int P = D / 16, ALL = SH::KEYS * P;  // pieces of a row, of the tile
+  const int blocks_in_page = (c.page_size >> 4) - 1;
+  uint8_t *raw = smem + SH::RAW_OFF + part * SH::KEYS * D;
+  KvWalk<SH::RT, SH::KEYS> ld = w;
+  int ld_j = ld.b;
+  const auto entry = [&] {
+    return ld.left > 0 ? kv_entry(c, bt, ld.s, ld_j * 8 + (lane & 7), ld.q.len) : -1;
+  };
+  int32_t ld_page = entry();
+  float sk = 0.0f, sv = 0.0f;  // lane i < 8: scales of block i, on their way until the tile is put
+  bool has = false;
+  const uint32_t page_bytes = static_cast<uint32_t>(c.page_bytes());
+  const auto fetch = [&] {
+    if (ld.left <= 0) return;
+    has = kv_page_ok(c, ld_page, ld_j * 8 + (lane & 7), ld.q.len);
+    const int32_t page = has ? ld_page : 0;  // (the mask hides a block without a page)
+    const uint32_t head = static_cast<uint32_t>((part * c.kv_heads + ld.head) * c.page_size) * D;
+#pragma unroll 4
+    for (int id = t; id < (ALL + N - 1) / N * N; id += N) {
+      const int row = id / P;  // (the shuffle takes every lane; pieces past the tile are dropped)
+      const int32_t pg = __shfl_sync(0xffffffffu, page, (row >> 4) & 7);
+      const uint32_t off = head + ((ld_j * 8 + (row >> 4)) & blocks_in_page) * (16 * D) + (row & 15) * D + id % P * 16;
+      if (ALL % N == 0 || id < ALL)
+        cp_async16(raw + id * 16, c.codes + static_cast<uint64_t>(static_cast<uint32_t>(pg)) * page_bytes + off);
+    }
+    if (part == 0 && t < 8) {
+      const int blk = (ld_j * 8 + t) & blocks_in_page;
+      sk = *c.scale(page, 0, ld.head, blk);
+      sv = *c.scale(page, 1, ld.head, blk);
+    }
+    if (++ld_j >= ld.e) {
+      ld.next(c, bt, a);
+      ld_j = ld.b;
+    }
+    ld_page = entry();
+  };
+  const float fscale = fabsf(a.scale_log2);
+  const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
+  uint64_t *empty = part == 0 ? bar->k_empty : bar->v_empty, *full = part == 0 ? bar->k_full : bar->v_full;
+  fetch();
+  cp_async_commit();
+  for (uint32_t n = 0; n < total; ++n) {
+    const int st = n & 1;
+    // a fresh barrier passes for its first use
+    if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], ((n >> 1) & 1) ^ 1))) break;
+    if (part == 0 && t < 32) {
+      // the slot's last readers are past: tile n - 2's scores, complete here, were issued after the
+      // softmax of tile n - 3, and the slot held tile n - 4
+      KpFactors *f = reinterpret_cast<KpFactors *>(smem + SH::F_OFF + (n & 3) * 80);
+      const uint32_t blocks = __ballot_sync(0xffffffffu, has) & 0xFFu;
+      if (lane < 8) f->k[lane] = has ? sk * fscale : 0.0f, f->v[lane] = has ? sv : 0.0f;
+      if (lane == 0) f->blocks = blocks;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->f_full[n & 3]);
+    }
+    cp_async_wait<0>();
+    uint8_t *tile = smem + (part == 0 ? SH::K_OFF : SH::V_OFF) + st * SH::TILE;
+#pragma unroll 2
+    for (int id = t; id < ALL; id += N) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(raw + id * 16);
+      const int row = id / P, pcol = id % P;
+      const uint2 b0 = bf16x4_of_bytes(v.x), b1 = bf16x4_of_bytes(v.y);
+      const uint2 b2 = bf16x4_of_bytes(v.z), b3 = bf16x4_of_bytes(v.w);
+      uint8_t *at = tile + (pcol >> 2) * SH::SUB + row * 128;
+      const int ch = (pcol & 3) * 2;
+      const uint4 lo = make_uint4(b0.x, b0.y, b1.x, b1.y), hi = make_uint4(b2.x, b2.y, b3.x, b3.y);
+      // lanes of the second sub-tile store their halves in the other order: no bank is hit twice
+      const bool sw = pcol & 4;
+      *reinterpret_cast<uint4 *>(at + (((ch + sw) ^ (row & 7)) << 4)) = sw ? hi : lo;
+      *reinterpret_cast<uint4 *>(at + (((ch + 1 - sw) ^ (row & 7)) << 4)) = sw ? lo : hi;
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(&full[st]);
+    fetch();
+    cp_async_commit();
+  }
+  cp_async_wait<0>();
+}
+
 template <int D>
 __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
     kv_prefill_kernel(KvCache c, KvBatch bt, KvAttn a, int min_blocks) {
@@ -159,13 +249,13 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
     mbar_init(&bar->q_ready, 256);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->k_full[i], 128), mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 128), mbar_init(&bar->v_empty[i], 1);
+      mbar_init(&bar->v_full[i], 96), mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 1), mbar_init(&bar->p_ready[i], 128), mbar_init(&bar->o_done[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bar->f_full[i], 1);
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 15) {
     tmem_alloc(&bar->tmem, 512);
     tmem_relinquish();
   }
@@ -179,7 +269,7 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
   pdl_trigger();  // the next kernel comes up only now that this one has its tensor memory
   if (!busy) {
     if (tid == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    if (warp == 12) tmem_dealloc(bar->tmem, 512);
+    if (warp == 15) tmem_dealloc(bar->tmem, 512);
     return;
   }
   const uint32_t tmem = bar->tmem;
@@ -262,68 +352,66 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
           const uint32_t in = n == 32 ? 0xFFFFFFFFu : (1u << n) - 1;
           return in & ((blocks >> (2 * h) & 1) * 0xFFFFu | (blocks >> (2 * h + 1) & 1) * 0xFFFF0000u);
         };
-        uint32_t s[2][32];
-        // ---- the tile's maximum
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int h = 0; h < 4; h += 2) {
-          tmem_ld_32x32b_x32(t_s + h * 32, s[0]);
-          tmem_ld_32x32b_x32(t_s + h * 32 + 32, s[1]);
-          tmem_ld_wait_regs(s[0]);
-          tmem_regs_after_wait(s[1]);
-          if (cut) {
-            const uint32_t k0 = keep(h), k1 = keep(h + 1);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if ((k0 >> i & 1) == 0) s[0][i] = 0xFF800000u;  // -inf
-              if ((k1 >> i & 1) == 0) s[1][i] = 0xFF800000u;
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            float v = __uint_as_float(s[b >> 1][(b & 1) * 16]);
-#pragma unroll
-            for (int i = 1; i < 16; ++i) v = fmaxf(v, __uint_as_float(s[b >> 1][(b & 1) * 16 + i]));
-            top = fmaxf(top, v * f->k[h * 2 + b]);
-          }
-        }
-        if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-          const float mn = fmaxf(m, top), g = ex2(m - mn);
+        // Moves this row's reference to its scores so far, `over` above it, before keys 32 h and on: the sums,
+        // the weights of the keys before (exactly: by a power of two) and O follow.
+        const auto move = [&](int h, float over) {
+          const bool known = m > -1e30f;
+          const float mn = known ? m + fmaxf(ceilf(over), 0.0f) : fmaxf(ceilf(over), -1e30f);
+          const float g = known ? ex2(m - mn) : 0.0f;
           m = mn;
           l2.x *= g, l2.y *= g;
+          tmem_st_wait();
+#pragma unroll 1
+          for (int i = 0; i < h; ++i) {
+            uint32_t p[16];
+            tmem_ld_32x32b_x16(t_s + i * 16, p);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              p[k] = pack_bf16x2(__uint_as_float(p[k] << 16) * g, __uint_as_float(p[k] & 0xFFFF0000u) * g);
+            tmem_st_32x32b_x16(t_s + i * 16, p);
+          }
           if (j > w.b) {
             // the products so far have been added up; the next ones wait for this tile's weights
-            ok = __all_sync(0xffffffffu, mbar_wait(&bar->o_done[x], (n_o + 1) & 1));
-            if (!ok) break;
+            ok = __all_sync(0xffffffffu, mbar_wait(&bar->o_done[x], (n_o + 1) & 1)) && ok;
             tc_fence_after();
 #pragma unroll 1
-            for (int h = 0; h < D / 32; ++h) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(t_o + h * 32, o);
-              tmem_ld_wait_regs(o);
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(t_o + i * 16, o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
-              tmem_st_32x32b_x32(t_o + h * 32, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * g);
+              tmem_st_32x32b_x16(t_o + i * 16, o);
             }
           }
-        }
-        // ---- weights: a second pass over the scores (holding all 128 would spill), the next 32 under way
-        // while these are worked on
+        };
+        // ---- weights of keys 32 h and on.  The reference stays as long as no score exceeds it by 2^8.
         const auto weights = [&](int h, uint32_t (&s)[32]) {
           float2 t[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float fk = f->k[h * 2 + (i >> 3)];
-            t[i] = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
-                        make_float2(fk, fk), make_float2(-m, -m));
-          }
-          if (cut) {  // (a factor of 0 would make -inf a NaN: the mask comes after it)
-            const uint32_t k = keep(h);
+          const auto scores = [&](float m) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              if ((k >> (2 * i) & 1) == 0) t[i].x = -INFINITY;
-              if ((k >> (2 * i + 1) & 1) == 0) t[i].y = -INFINITY;
+              const float fk = f->k[h * 2 + (i >> 3)];
+              t[i] = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
+                          make_float2(fk, fk), make_float2(-m, -m));
             }
+            if (cut) {  // (a factor of 0 would make -inf a NaN: the mask comes after it)
+              const uint32_t k = keep(h);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                if ((k >> (2 * i) & 1) == 0) t[i].x = -INFINITY;
+                if ((k >> (2 * i + 1) & 1) == 0) t[i].y = -INFINITY;
+              }
+            }
+            float2 hi = t[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) hi.x = fmaxf(hi.x, t[i].x), hi.y = fmaxf(hi.y, t[i].y);
+            return fmaxf(hi.x, hi.y);
+          };
+          const bool known = m > -1e30f;
+          const float over = scores(known ? m : 0.0f);
+          if (__any_sync(0xffffffffu, known ? over > 8.0f : over > -INFINITY)) {
+            move(h, over);
+            scores(m > -1e30f ? m : 0.0f);
           }
           uint32_t p[16];
 #pragma unroll
@@ -334,19 +422,21 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
             const float2 wt = mul2(e, make_float2(fv, fv));
             p[i] = pack_bf16x2(wt.x, wt.y);
           }
-          tmem_st_32x32b_x16(t_s + h * 16, p);
+          tmem_st_32x32b_x16(t_s + h * 16, p);  // over scores already taken
         };
-        tmem_ld_32x32b_x32(t_s, s[0]);
-        tmem_ld_wait_regs(s[0]);
+        uint32_t s[32];
+        tmem_ld_32x32b_x32(t_s, s);
+        tmem_ld_wait_regs(s);
 #pragma unroll 1
-        for (int h = 0; h < 4; h += 2) {
-          tmem_ld_32x32b_x32(t_s + h * 32 + 32, s[1]);
-          weights(h, s[0]);
-          tmem_ld_wait_regs(s[1]);
-          if (h == 0) tmem_ld_32x32b_x32(t_s + 64, s[0]);
-          weights(h + 1, s[1]);
-          if (h == 0) tmem_ld_wait_regs(s[0]);
+        for (int h = 0; h < 4; ++h) {  // the next 32 scores are under way while these are worked on
+          uint32_t next[32];
+          tmem_ld_32x32b_x32(t_s + min(h + 1, 3) * 32, next);
+          weights(h, s);
+          tmem_ld_wait_regs(next);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = next[i];
         }
+        if (!ok) break;
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bar->p_ready[x]);
@@ -441,104 +531,12 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
       w.next(c, bt, a);
     }
   } else if (warp < 12) {
-    // ================================================================ codes -> bf16 tiles
-    // Thread t takes 16-byte piece t % P of row t / P of each 16-token block (P pieces a row, 2 blocks
-    // a pass at D = 64); a block's page is looked up once per tile.
-    const int t = tid - 256;
-    constexpr int P = D / 16, RPI = 128 / P, N = SH::KEYS / RPI;  // pieces, rows a pass, passes
-    const int prow = t / P, pcol = t % P;
-    const float fscale = fabsf(a.scale_log2);
-    uint32_t n = 0;
-    bool ok = true;
-    Walk ld = w;     // the tile whose codes are fetched next
-    int ld_j = ld.b;
-    const auto entry = [&] {  // lane i % 8: the table's entry for the tile's block i
-      return ld.left > 0 ? kv_entry(c, bt, ld.s, ld_j * 8 + (lane & 7), ld.q.len) : -1;
-    };
-    int32_t ld_page = entry();  // looked up a tile before it is used
-    float fk = 0.0f, fv = 0.0f;  // lane i < 8: factors of block i
-    bool has = false;
-    // The codes of the next tile come into each thread's own slots (no barrier), K and V a group each.
-    uint8_t *raw = smem + SH::RAW_OFF + t * 16;
-    const auto fetch = [&](int which) {
-      if (ld.left <= 0) return;
-      const bool ok_page = kv_page_ok(c, ld_page, ld_j * 8 + (lane & 7), ld.q.len);
-      const int32_t page = ok_page ? ld_page : 0;  // (the mask hides a block without a page)
-#pragma unroll 2
-      for (int i = 0; i < N; ++i) {
-        const int row = i * RPI + prow;
-        const int8_t *p = c.block(__shfl_sync(0xffffffffu, page, row >> 4), which, ld.head,
-                                  (ld_j * 8 + (row >> 4)) & ((c.page_size >> 4) - 1)) + (row & 15) * D + pcol * 16;
-        cp_async16(raw + (which * N + i) * 2048, p);
-      }
-      if (which == 0) return;
-      has = ok_page;
-      if (t < 8) {
-        const int blk = (ld_j * 8 + t) & ((c.page_size >> 4) - 1);
-        fk = has ? *c.scale(page, 0, ld.head, blk) * fscale : 0.0f;
-        fv = has ? *c.scale(page, 1, ld.head, blk) : 0.0f;
-      }
-      if (++ld_j >= ld.e) {
-        ld.next(c, bt, a);
-        ld_j = ld.b;
-      }
-      ld_page = entry();
-    };
-    const auto put = [&](uint8_t *tile, int which) {
-      cp_async_wait<1>();
-#pragma unroll 2
-      for (int i = 0; i < N; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(raw + (which * N + i) * 2048);
-        const int row = i * RPI + prow;
-        const uint2 b0 = bf16x4_of_bytes(v.x), b1 = bf16x4_of_bytes(v.y);
-        const uint2 b2 = bf16x4_of_bytes(v.z), b3 = bf16x4_of_bytes(v.w);
-        uint8_t *at = tile + (pcol >> 2) * SH::SUB + row * 128;
-        const int ch = (pcol & 3) * 2;
-        const uint4 lo = make_uint4(b0.x, b0.y, b1.x, b1.y), hi = make_uint4(b2.x, b2.y, b3.x, b3.y);
-        // lanes of the second sub-tile store their halves in the other order: no bank is hit twice
-        const bool sw = pcol & 4;
-        *reinterpret_cast<uint4 *>(at + (((ch + sw) ^ (row & 7)) << 4)) = sw ? hi : lo;
-        *reinterpret_cast<uint4 *>(at + (((ch + 1 - sw) ^ (row & 7)) << 4)) = sw ? lo : hi;
-      }
-      fence_proxy_async_smem();
-    };
-    const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
-    // A tile's K is fetched while V of the tile before is converted: fetch(0) of the next tile needs that
-    // tile's entries, which fetch(1) of this one looked up
-    fetch(0);
-    cp_async_commit();
-    fetch(1);
-    cp_async_commit();
-    for (; n < total; ++n) {
-      const int st = n & 1;
-      // a fresh barrier passes for its first use
-      ok = __all_sync(0xffffffffu, mbar_wait(&bar->k_empty[st], ((n >> 1) & 1) ^ 1));
-      if (!ok) break;
-      if (warp == 8) {
-        // the slot's last readers are past: tile n - 2's scores, complete here, were issued after the
-        // softmax of tile n - 3, and the slot held tile n - 4
-        KpFactors *f = reinterpret_cast<KpFactors *>(smem + SH::F_OFF + (n & 3) * 80);
-        const uint32_t blocks = __ballot_sync(0xffffffffu, has) & 0xFFu;
-        if (lane < 8) f->k[lane] = fk, f->v[lane] = fv;
-        if (lane == 0) f->blocks = blocks;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar->f_full[n & 3]);
-      }
-      put(smem + SH::K_OFF + st * SH::TILE, 0);
-      mbar_arrive(&bar->k_full[st]);
-      fetch(0);
-      cp_async_commit();
-      ok = __all_sync(0xffffffffu, mbar_wait(&bar->v_empty[st], ((n >> 1) & 1) ^ 1));
-      if (!ok) break;
-      put(smem + SH::V_OFF + st * SH::TILE, 1);
-      mbar_arrive(&bar->v_full[st]);
-      fetch(1);
-      cp_async_commit();
-    }
-    cp_async_wait<0>();
+    kv_prefill_codes<D, 0, 128>(c, bt, a, w, smem, bar, tid - 256);
   } else {
-    set_registers_down<SH::R_ISSUE>();
-    if (warp == 12 && lane == 0) {
+    set_registers_down<SH::R_REST>();
+    if (warp < 15) {
+      kv_prefill_codes<D, 1, 96>(c, bt, a, w, smem, bar, tid - 384);
+    } else if (lane == 0) {
     // ================================================================ MMA issue
     const uint32_t q0 = smem_u32(smem + SH::Q_OFF), k0 = smem_u32(smem + SH::K_OFF), v0 = smem_u32(smem + SH::V_OFF);
     uint32_t n = 0, n_q = 0, n_p[2] = {0, 0};
@@ -599,7 +597,7 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 15) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace rt
