@@ -161,7 +161,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle of torch.cuda.current_stream(t.device), without building a Stream object per call
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def device_status(device: torch.device, *, clear: bool = True) -> int:

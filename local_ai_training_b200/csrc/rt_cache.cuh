@@ -102,16 +102,18 @@ struct KvNew {
   int head_dim;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31;
+// What one warp appends: rows [p0, p1) of a block are new (rows before p0 were held).
+struct KvPiece {
+  int8_t *dst;   // the block's codes
+  float *scale;
+  int64_t row;   // the call's row at the block's row 0 (before the first new one: not read)
+  int part, head, p0, p1;
+};
+__device__ __forceinline__ bool kv_append_piece(const KvCache &c, const KvBatch &b, int slots, KvPiece &x) {
   const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int per = 2 * c.kv_heads;
-  const int slot = static_cast<int>(w / per), part = static_cast<int>(w % per) / c.kv_heads;
-  const int head = static_cast<int>(w % c.kv_heads);
-  if (slot >= slots) return;
+  const int slot = static_cast<int>(w / per), rest = static_cast<int>(w % per);
+  if (slot >= slots) return false;
   int64_t lo = 0, hi = b.n_seqs;  // last s whose first slot is <= slot
   while (lo + 1 < hi) {
     const int64_t mid = (lo + hi) >> 1;
@@ -121,22 +123,38 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, Kv
       hi = mid;
   }
   const KvSeq q = kv_seq(b, c.page_size, lo);
-  if (q.n == 0) return;
+  if (q.n == 0) return false;
   const int blk = (max(q.start, 0) >> 4) + slot - ((q.c0 >> 4) + 2 * static_cast<int>(lo));
-  if (blk * KV_BLOCK >= q.len || blk < 0) return;
+  if (blk * KV_BLOCK >= q.len || blk < 0) return false;
   const int64_t page = kv_page(c, b, lo, blk);
-  if (page < 0) return;
+  if (page < 0) return false;
   const int in_page = blk & ((c.page_size >> 4) - 1);
-  int8_t *dst = c.block(page, part, head, in_page);
-  float *sp = c.scale(page, part, head, in_page);
-  const int p0 = max(q.start - blk * KV_BLOCK, 0);            // first new row
-  const int p1 = min(q.len - blk * KV_BLOCK, KV_BLOCK);       // rows of the block in use
-  const int64_t st = part == 0 ? x.k_token : x.v_token, sh = part == 0 ? x.k_head : x.v_head;
-  const T *src = static_cast<const T *>(part == 0 ? x.k : x.v) +
-                 (q.c0 + static_cast<int64_t>(blk) * KV_BLOCK - q.start) * st + head * sh;
+  x.part = rest >= c.kv_heads, x.head = rest - x.part * c.kv_heads;
+  x.dst = c.block(page, x.part, x.head, in_page);
+  x.scale = c.scale(page, x.part, x.head, in_page);
+  x.p0 = max(q.start - blk * KV_BLOCK, 0);
+  x.p1 = min(q.len - blk * KV_BLOCK, KV_BLOCK);
+  x.row = q.c0 + static_cast<int64_t>(blk) * KV_BLOCK - q.start;
+  return true;
+}
+__device__ __forceinline__ int8_t kv_code(float v, float s) {
+  const float q = v != v ? 0.0f : fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
+  return static_cast<int8_t>(static_cast<int>(q));
+}
+
+// Any strides and widths: the rows are read twice, the second time from the cache.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_append_any_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  KvPiece p;
+  if (!kv_append_piece(c, b, slots, p)) return;
+  const int64_t st = p.part == 0 ? x.k_token : x.v_token, sh = p.part == 0 ? x.k_head : x.v_head;
+  const T *src = static_cast<const T *>(p.part == 0 ? x.k : x.v) + p.row * st + p.head * sh;
   float amax = 0.0f;
   bool odd = false;
-  for (int r = p0; r < p1; ++r)
+  for (int r = p.p0; r < p.p1; ++r)
     for (int d = lane; d < x.head_dim; d += 32) {
       const float a = fabsf(load_as_float(src + r * st + d));
       if (a <= FLT_MAX)
@@ -146,24 +164,133 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, Kv
     }
   amax = warp_max(amax);
   if (odd) raise_status(RT_STATUS_NONFINITE_KV);
-  const float old = p0 > 0 ? *sp : 0.0f;
+  const float old = p.p0 > 0 ? *p.scale : 0.0f;
   const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
-  if (p0 > 0 && s > old) {
+  if (p.p0 > 0 && s > old) {
     const float ratio = __fdiv_rn(old, s);
-    for (int i = lane; i < p0 * c.dim; i += 32)
-      dst[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(dst[i]), ratio)));
+    for (int i = lane; i < p.p0 * c.dim; i += 32)
+      p.dst[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(p.dst[i]), ratio)));
   }
-  for (int r = p0; r < p1; ++r)
-    for (int d = lane; d < c.dim; d += 32) {
-      float q8 = 0.0f;
-      if (d < x.head_dim) {
-        const float v = load_as_float(src + r * st + d);
-        q8 = v != v ? 0.0f : fminf(fmaxf(rintf(__fdiv_rn(v, s)), -127.0f), 127.0f);
+  for (int r = p.p0; r < p.p1; ++r)
+    for (int d = lane; d < c.dim; d += 32)
+      p.dst[r * c.dim + d] = d < x.head_dim ? kv_code(load_as_float(src + r * st + d), s) : 0;
+  __syncwarp();
+  if (lane == 0) *p.scale = s;
+}
+
+// Rows of whole stored width in 16-byte accesses: a block's new rows are read once and stay in registers.
+// Bound by HBM (the element's bytes read, one written); the division is replaced by a product with
+// 1 / s where that rounds to the same code, which it does unless x / s lies within 2^-15 of the middle
+// between two codes (both are within 127 · 1.5 · 2^-23 of the exact quotient); those elements, a few in
+// 10^5, are divided.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
+  constexpr int E = 16 / sizeof(T);          // elements of an access
+  constexpr int LPR = D / E < 32 ? D / E : 32;  // lanes of a row
+  constexpr int RPP = 32 / LPR;              // rows of a pass
+  constexpr int CH = D / (E * LPR);          // accesses of a lane and row
+  constexpr int PASSES = KV_BLOCK / RPP;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  KvPiece p;
+  if (!kv_append_piece(c, b, slots, p)) return;
+  const int64_t st = p.part == 0 ? x.k_token : x.v_token, sh = p.part == 0 ? x.k_head : x.v_head;
+  const int r0 = lane / LPR, col = lane % LPR * E;
+  const T *src = static_cast<const T *>(p.part == 0 ? x.k : x.v) + p.row * st + p.head * sh + col;
+  uint4 v[PASSES * CH];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int r = r0 + i * RPP;
+      v[i * CH + k] = make_uint4(0, 0, 0, 0);
+      if (r >= p.p0 && r < p.p1)
+        v[i * CH + k] = __ldcs(reinterpret_cast<const uint4 *>(src + r * st + k * LPR * E));
+    }
+  const float old = p.p0 > 0 ? *p.scale : 0.0f;
+  const auto element = [&](const uint4 &u, int e) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+  };
+  uint32_t top = 0;  // |x| as bits: order and all, with infinity and NaN above every number
+#pragma unroll
+  for (int i = 0; i < PASSES * CH; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(element(v[i], e)) & 0x7FFFFFFFu);
+  float amax = __uint_as_float(top);
+  bool odd = top >= 0x7F800000u;
+  if (__any_sync(0xffffffffu, odd)) {
+    if (odd) raise_status(RT_STATUS_NONFINITE_KV);
+    odd = true;
+    amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PASSES * CH; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float a = fabsf(element(v[i], e));
+        if (a <= FLT_MAX) amax = fmaxf(amax, a);
       }
-      dst[r * c.dim + d] = static_cast<int8_t>(static_cast<int>(q8));
+  }
+  amax = warp_max(amax);
+  const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
+  if (p.p0 > 0 && s > old) {
+    const float ratio = __fdiv_rn(old, s);
+    for (int i = lane; i < p.p0 * (D / 4); i += 32) {
+      char4 *at = reinterpret_cast<char4 *>(p.dst) + i;
+      char4 q = *at;
+      q.x = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.x), ratio)));
+      q.y = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.y), ratio)));
+      q.z = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.z), ratio)));
+      q.w = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.w), ratio)));
+      *at = q;
+    }
+  }
+  const float inv = __fdiv_rn(1.0f, s);
+  const bool divide = odd || s > 1e37f;  // (1 / s must be a normal number)
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const uint4 u = v[i * CH + k];
+      uint32_t code[E / 4];
+      float off = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // 1.5 · 2^23 + rint(x / s): the code is the low byte
+          const float y = __fmaf_rn(element(u, e + j), inv, 12582912.0f);
+          off = fmaxf(off, fabsf(__fmaf_rn(element(u, e + j), inv, 12582912.0f - y)));
+          q[j] = __float_as_uint(y);
+        }
+        code[e / 4] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+      }
+      if (divide || off > 0.5f - 3.0517578125e-5f) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          uint32_t w = 0;
+#pragma unroll 1
+          for (int j = 3; j >= 0; --j) {
+            const float f = j == 0 ? element(u, e) : j == 1 ? element(u, e + 1) : j == 2 ? element(u, e + 2) : element(u, e + 3);
+            w = w << 8 | static_cast<uint8_t>(kv_code(f, s));
+          }
+          code[e / 4] = w;
+        }
+      }
+      const int r = r0 + i * RPP;
+      if (r >= p.p0 && r < p.p1) {
+        uint32_t *dst = reinterpret_cast<uint32_t *>(p.dst + r * D + k * LPR * E + col);
+        if constexpr (E == 8)
+          *reinterpret_cast<uint2 *>(dst) = make_uint2(code[0], code[1]);
+        else
+          *dst = code[0];
+      }
     }
   __syncwarp();
-  if (lane == 0) *sp = s;
+  if (lane == 0) *p.scale = s;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -178,26 +305,73 @@ __device__ __forceinline__ void store_from_float<__nv_bfloat16>(__nv_bfloat16 *p
   *p = __float2bfloat16_rn(v);
 }
 
+// Four rows per CTA; `vec`: whole stored widths and 16-byte aligned outputs, 16 codes per access.
+constexpr int KR_ROWS = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
-    kv_read_kernel(KvCache c, KvBatch b, int head_dim, T *k_out, T *v_out) {
+    kv_read_kernel(KvCache c, KvBatch b, int head_dim, bool vec, T *k_out, T *v_out) {
   pdl_wait();
   pdl_trigger();
-  const int64_t t = blockIdx.x;
-  const int64_t s = kv_seq_of(b.cu, b.n_seqs, t);
-  const int64_t pos = s < 0 ? -1 : __ldg(b.kv_lens + s) + t - __ldg(b.cu + s);
-  const bool in = pos >= 0 && pos < b.pages_per_seq * c.page_size;
-  if (s >= 0 && !in) raise_status(RT_STATUS_INDEX_RANGE);
-  const int64_t page = in ? kv_page(c, b, s, static_cast<int>(pos >> 4)) : -1;
-  const int row = static_cast<int>(pos & 15), blk = static_cast<int>(pos >> 4) & ((c.page_size >> 4) - 1);
-  const int n = c.kv_heads * head_dim;
-  for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
-    const int part = i >= n, j = i - part * n, h = j / head_dim, d = j % head_dim;
-    float v = 0.0f;
-    if (page >= 0)
-      v = __fmul_rn(static_cast<float>(c.block(page, part, h, blk)[row * c.dim + d]),
-                    *c.scale(page, part, h, blk));
-    store_from_float((part ? v_out : k_out) + t * n + j, v);
+  __shared__ int64_t sm_page[KR_ROWS];
+  __shared__ int sm_pos[KR_ROWS];
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * KR_ROWS;
+  if (threadIdx.x < KR_ROWS && t0 + threadIdx.x < b.n_tokens) {
+    const int64_t t = t0 + threadIdx.x, s = kv_seq_of(b.cu, b.n_seqs, t);
+    const int64_t pos = s < 0 ? -1 : __ldg(b.kv_lens + s) + t - __ldg(b.cu + s);
+    const bool in = pos >= 0 && pos < b.pages_per_seq * c.page_size;
+    if (s >= 0 && !in) raise_status(RT_STATUS_INDEX_RANGE);
+    sm_page[threadIdx.x] = in ? kv_page(c, b, s, static_cast<int>(pos >> 4)) : -1;
+    sm_pos[threadIdx.x] = static_cast<int>(pos);
+  }
+  __syncthreads();
+  const int rows = static_cast<int>(min(static_cast<int64_t>(KR_ROWS), b.n_tokens - t0));
+  const int step = vec ? 16 : 1, per = c.kv_heads * head_dim / step;  // accesses of a row's K or V
+  const int mask = (c.page_size >> 4) - 1;
+  for (int i = threadIdx.x; i < 2 * per; i += 256) {
+    const int part = i >= per, j = (i - part * per) * step, h = j / head_dim, d = j - h * head_dim;
+    T *out = (part ? v_out : k_out) + t0 * c.kv_heads * head_dim + j;
+    if (vec) {
+      uint4 q[KR_ROWS];
+      float s[KR_ROWS];
+#pragma unroll
+      for (int r = 0; r < KR_ROWS; ++r) {
+        const bool in = r < rows && sm_page[r] >= 0;
+        const int blk = (sm_pos[r] >> 4) & mask;
+        q[r] = in ? __ldg(reinterpret_cast<const uint4 *>(c.block(sm_page[r], part, h, blk) + (sm_pos[r] & 15) * c.dim + d))
+                  : make_uint4(0, 0, 0, 0);
+        s[r] = in ? __ldg(c.scale(sm_page[r], part, h, blk)) : 0.0f;
+      }
+#pragma unroll
+      for (int r = 0; r < KR_ROWS; ++r) {
+        if (r >= rows) break;
+        const uint32_t w[4] = {q[r].x, q[r].y, q[r].z, q[r].w};
+        uint4 *o = reinterpret_cast<uint4 *>(out + static_cast<int64_t>(r) * c.kv_heads * head_dim);
+        uint32_t f[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          f[k] = __float_as_uint(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[k >> 2] >> (k & 3) * 8)), s[r]));
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) __stcs(o + k, make_uint4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]));
+        } else {
+          uint32_t p[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) p[k] = pack_bf16x2(__uint_as_float(f[2 * k]), __uint_as_float(f[2 * k + 1]));
+          __stcs(o, make_uint4(p[0], p[1], p[2], p[3]));
+          __stcs(o + 1, make_uint4(p[4], p[5], p[6], p[7]));
+        }
+      }
+    } else {
+      for (int r = 0; r < rows; ++r) {
+        float v = 0.0f;
+        if (sm_page[r] >= 0) {
+          const int blk = (sm_pos[r] >> 4) & mask;
+          v = __fmul_rn(static_cast<float>(c.block(sm_page[r], part, h, blk)[(sm_pos[r] & 15) * c.dim + d]),
+                        *c.scale(sm_page[r], part, h, blk));
+        }
+        store_from_float(out + static_cast<int64_t>(r) * c.kv_heads * head_dim, v);
+      }
+    }
   }
 }
 
@@ -305,13 +479,22 @@ extern "C" int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t
   const int64_t slots = n_tokens / KV_BLOCK + 2 * n_seqs;
   const int64_t grid = (slots * 2 * kv_heads + 7) / 8;
   if (grid > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "kv_append: batch too large");
-  cudaStream_t s = as_stream(stream);
+  const int es = dtype == RT_F32 ? 4 : 2;
+  const bool vec = head_dim == padded_dim && aligned16(k) && aligned16(v) && k_stride_token * es % 16 == 0 &&
+                   k_stride_head * es % 16 == 0 && v_stride_token * es % 16 == 0 &&
+                   v_stride_head * es % 16 == 0;
+  // (an fp32 block of width 256 does not fit a warp's registers)
+  const auto kernel = [&](auto *any, auto *d32, auto *d64, auto *d128, auto *d256) {
+    auto *f = !vec ? any : padded_dim == 32 ? d32 : padded_dim == 64 ? d64 : padded_dim == 128 ? d128 : d256;
+    launch_k(f, static_cast<unsigned>(grid), 256, 0, as_stream(stream), c, b, x, static_cast<int>(slots));
+  };
   if (dtype == RT_F32)
-    launch_k(kv_append_kernel<float>, static_cast<unsigned>(grid), 256, 0, s, c, b, x,
-             static_cast<int>(slots));
+    kernel(kv_append_any_kernel<float>, kv_append_kernel<float, 32>, kv_append_kernel<float, 64>,
+           kv_append_kernel<float, 128>, kv_append_any_kernel<float>);
   else
-    launch_k(kv_append_kernel<__nv_bfloat16>, static_cast<unsigned>(grid), 256, 0, s, c, b, x,
-             static_cast<int>(slots));
+    kernel(kv_append_any_kernel<__nv_bfloat16>, kv_append_kernel<__nv_bfloat16, 32>,
+           kv_append_kernel<__nv_bfloat16, 64>, kv_append_kernel<__nv_bfloat16, 128>,
+           kv_append_kernel<__nv_bfloat16, 256>);
   return check_launch("kv_append");
 }
 
@@ -334,12 +517,13 @@ extern "C" int rt_kv_read(const void *codes, const float *scales, int64_t n_page
   if (k_out == nullptr || v_out == nullptr)
     return fail(RT_ERR_INVALID_ARGUMENT, "kv_read: null pointer");
   cudaStream_t s = as_stream(stream);
-  const unsigned grid = static_cast<unsigned>(n_tokens);
+  const unsigned grid = static_cast<unsigned>((n_tokens + KR_ROWS - 1) / KR_ROWS);
+  const bool vec = head_dim == padded_dim && aligned16(k_out) && aligned16(v_out);
   if (dtype == RT_F32)
-    launch_k(kv_read_kernel<float>, grid, 256, 0, s, c, b, static_cast<int>(head_dim),
+    launch_k(kv_read_kernel<float>, grid, 256, 0, s, c, b, static_cast<int>(head_dim), vec,
              static_cast<float *>(k_out), static_cast<float *>(v_out));
   else
-    launch_k(kv_read_kernel<__nv_bfloat16>, grid, 256, 0, s, c, b, static_cast<int>(head_dim),
+    launch_k(kv_read_kernel<__nv_bfloat16>, grid, 256, 0, s, c, b, static_cast<int>(head_dim), vec,
              static_cast<__nv_bfloat16 *>(k_out), static_cast<__nv_bfloat16 *>(v_out));
   return check_launch("kv_read");
 }

@@ -131,8 +131,10 @@ struct KvWalk {
     tiles = rows >= a.rows_lo && rows < a.rows_hi ? (rows + RT - 1) / RT : 0;
   }
   // Blocks of sequence s over all its row tiles (one kv head).
-  __device__ __forceinline__ int64_t seq_blocks(const KvCache &c, const KvBatch &bt, const KvAttn &a) {
+  __device__ __forceinline__ int64_t seq_blocks(const KvCache &c, const KvBatch &bt, const KvAttn &a,
+                                                bool units = false) {
     set_seq(c, bt, a);
+    if (units) return tiles;  // units instead of blocks
     int64_t sum = 0;
     for (tile = 0; tile < tiles; ++tile) {
       set_tile(a);
@@ -164,7 +166,8 @@ struct KvWalk {
 };
 
 // Sets this CTA's share of the line: all of the grid has equal shares of a long line, and as many CTAs as
-// get min_blocks each of a short one.  Returns false (for every thread) when this CTA has none.
+// get min_blocks each of a short one.  With min_blocks = 0 a CTA takes one whole unit (the grid has one
+// for each), so no rows are left to join.  Returns false (for every thread) when this CTA has no share.
 template <int THREADS, int RT, int KEYS>
 __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache &c, const KvBatch &bt,
                                               const KvAttn &a, int min_blocks) {
@@ -172,11 +175,12 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
   __shared__ int64_t sm_sum[WARPS];
   __shared__ int sm_start[5];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool units = min_blocks == 0;
   const int per = static_cast<int>((bt.n_seqs + THREADS - 1) / THREADS);
   const int s0 = min(tid * per, static_cast<int>(bt.n_seqs));
   const int s1 = min(s0 + per, static_cast<int>(bt.n_seqs));
   int64_t mine = 0;
-  for (w.s = s0; w.s < s1; ++w.s) mine += w.seq_blocks(c, bt, a);
+  for (w.s = s0; w.s < s1; ++w.s) mine += w.seq_blocks(c, bt, a, units);
   mine *= c.kv_heads;
   int64_t scan = mine;
 #pragma unroll
@@ -193,26 +197,27 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
     if (i < warp) before += sm_sum[i];
     total += sm_sum[i];
   }
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), (total + min_blocks - 1) / min_blocks);
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), units ? total : (total + min_blocks - 1) / min_blocks);
   const int64_t p0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
   const int64_t p1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
   if (p0 < p1 && before <= p0 && p0 < before + mine) {  // one thread's sequences hold p0
     int64_t at = before;
     for (w.s = s0; w.s < s1 - 1; ++w.s) {
-      const int64_t n = w.seq_blocks(c, bt, a) * c.kv_heads;
+      const int64_t n = w.seq_blocks(c, bt, a, units) * c.kv_heads;
       if (p0 < at + n) break;
       at += n;
     }
     w.set_seq(c, bt, a);
     for (w.tile = 0;; ++w.tile) {
       w.set_tile(a);
-      const int64_t n = static_cast<int64_t>(w.nb) * c.kv_heads;
+      const int64_t n = static_cast<int64_t>(units ? 1 : w.nb) * c.kv_heads;
       if (p0 < at + n || w.tile >= w.tiles - 1) break;
       at += n;
     }
+    const int per_head = units ? 1 : w.nb;
     sm_start[0] = w.s, sm_start[1] = w.tile;
-    sm_start[2] = static_cast<int>((p0 - at) / w.nb), sm_start[3] = static_cast<int>((p0 - at) % w.nb);
-    sm_start[4] = static_cast<int>(p1 - p0);
+    sm_start[2] = static_cast<int>((p0 - at) / per_head), sm_start[3] = static_cast<int>((p0 - at) % per_head);
+    sm_start[4] = units ? w.nb : static_cast<int>(p1 - p0);
   }
   __syncthreads();
   if (sm_start[0] < 0) return false;
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
   kv_zero_rest<T>(bt, a);
   KvWalk<RT, KV_BLOCK> w;
   if (!kv_walk_start<KA_WARPS * 32>(w, c, bt, a, min_blocks)) {
-    if (tid == 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && min_blocks != 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
 
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
         if (d == 0) dst[0] = top, dst[1] = den;
       }
     }
-    if (tid == 0) {
+    if (tid == 0 && min_blocks != 0) {
       int4 *mt = a.meta + blockIdx.x;
       if (first_piece) *mt = make_int4(-1, 0, 0, 0);
       if (w.b > 0) mt->w = w.e == w.nb;

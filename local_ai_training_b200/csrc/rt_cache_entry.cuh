@@ -1,6 +1,8 @@
 // rt_cache_entry.cuh — the attention entry point: which kernels a batch takes, their grids and workspace.
 #pragma once
 
+#include <algorithm>
+
 #include "rt_cache_prefill.cuh"
 
 namespace rt {
@@ -43,7 +45,18 @@ int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int s
   static bool done[64] = {false};
   auto *kernel = kv_attention_kernel<T, D, NT>;
   if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
+  // Few and short units: one CTA each and no join, whose launch costs more than the 8 blocks, at most, that
+  // each warp then takes.  Row tiles of a batch, at most: a partly filled one per sequence with rows,
+  // and one per token while a token's rows fit a tile.
+  const int64_t rows = bt.n_tokens * a.group, some = std::min(bt.n_tokens, bt.n_seqs);
+  int64_t units = (rows + some * (SH::RT - 1)) / SH::RT;
+  if (a.group <= SH::RT) units = std::min(units, bt.n_tokens);
+  units *= c.kv_heads;
   const int ctas = sms * SH::MIN_CTAS;
+  if (units > 0 && units <= ctas && bt.pages_per_seq * c.page_size <= 64 * KV_BLOCK) {
+    launch_k(kernel, static_cast<unsigned>(units), KA_WARPS * 32, SH::SMEM, s, c, bt, a, 0);
+    return check_launch("kv_attention");
+  }
   launch_k(kernel, ctas, KA_WARPS * 32, SH::SMEM, s, c, bt, a, KA_WARPS);
   launch_k(kv_attention_join_kernel<T, D, SH::RT>, dim3(ctas, SH::RT / 8), 256, 0, s, c, bt,
            a, ctas);

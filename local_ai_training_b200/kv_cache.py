@@ -17,6 +17,7 @@ STATUS_INDEX_RANGE in the device status word.
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -38,31 +39,41 @@ def padded_head_dim(head_dim: int) -> int:
     raise ValueError("head_dim must be in [1, 256]")
 
 
-def _check_cache(codes: Tensor, scales: Tensor, what: str, ndim: int = 5) -> None:
+def _check_cache(codes: Tensor, scales: Tensor, what: str, ndim: int = 5):
+    """The cache's shape, checked.  (Decode calls are a few microseconds: each attribute is read once.)"""
     if not codes.is_cuda:
         raise RuntimeError(f"{what} requires CUDA; the key/value cache is GPU-only")
     if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise TypeError(f"{what}: codes must be int8 and scales float32")
     shape = codes.shape
-    if (codes.dim() != ndim or shape[-4] != 2
-            or scales.shape != shape[:-2] + (shape[-2] // QUANT_BLOCK,)):
+    if (len(shape) != ndim or shape[-4] != 2 or scales.dim() != ndim - 1
+            or scales.numel() * QUANT_BLOCK * shape[-1] != codes.numel()
+            or scales.shape[-1] * QUANT_BLOCK != shape[-2] or scales.shape[-2] != shape[-3]):
         raise ValueError(f"{what}: codes must be [..., pages, 2, heads, page_size, width] and scales "
                          "[..., pages, 2, heads, page_size / 16]")
     if not (codes.is_contiguous() and scales.is_contiguous()):
         raise ValueError(f"{what}: codes and scales must be contiguous")
+    return shape
 
 
-def _check_batch(page_table: Tensor, lens: Tensor, cu_tokens: Tensor, what: str) -> None:
+def _check_batch(page_table: Tensor, lens: Tensor, cu_tokens: Tensor, what: str) -> tuple[int, int]:
+    """(sequences, pages per sequence) of a batch, checked."""
     if not (page_table.dtype is lens.dtype is cu_tokens.dtype is torch.int32):
         raise TypeError(f"{what}: page_table, lengths and cu_tokens must be int32")
-    seqs = lens.numel()
-    if (page_table.dim() != 2 or page_table.shape[0] != seqs or cu_tokens.numel() != seqs + 1):
+    shape, seqs = page_table.shape, lens.numel()
+    if len(shape) != 2 or shape[0] != seqs or cu_tokens.numel() != seqs + 1:
         raise ValueError(f"{what}: page_table must be [seqs, pages], lengths [seqs] and cu_tokens "
                          "[seqs + 1]")
     if not (page_table.is_contiguous() and lens.is_contiguous() and cu_tokens.is_contiguous()):
         raise ValueError(f"{what}: page_table, lengths and cu_tokens must be contiguous")
     if not (page_table.is_cuda and lens.is_cuda and cu_tokens.is_cuda):
         raise RuntimeError(f"{what} requires CUDA; the batch is read on the device")
+    return seqs, shape[1]
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(seqs: int, tokens: int, heads: int, kv_heads: int, width: int, device: int) -> int:
+    return _lib.lib().rt_kv_attention_workspace_bytes(seqs, tokens, heads, kv_heads, width)
 
 
 def kv_append(codes: Tensor, scales: Tensor, page_table: Tensor, kv_lens: Tensor, cu_tokens: Tensor,
@@ -72,29 +83,31 @@ def kv_append(codes: Tensor, scales: Tensor, page_table: Tensor, kv_lens: Tensor
 
     A block's scale is max|x| / 127 over its tokens and only grows while its tokens arrive; codes
     already held are re-rounded when it does.  No two sequences may append into one page."""
-    _check_cache(codes, scales, "kv_append")
-    _check_batch(page_table, kv_lens, cu_tokens, "kv_append")
-    pages, _, heads, page_size, width = codes.shape
-    if k.shape != v.shape or k.dim() != 3 or k.shape[1] != heads or k.shape[2] > width:
+    pages, _, heads, page_size, width = _check_cache(codes, scales, "kv_append")
+    seqs, per_seq = _check_batch(page_table, kv_lens, cu_tokens, "kv_append")
+    shape = k.shape
+    if v.shape != shape or len(shape) != 3 or shape[1] != heads or shape[2] > width:
         raise ValueError("kv_append: k and v must be [tokens, kv_heads, head_dim] of the cache's heads")
     if k.dtype is not v.dtype or k.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("kv_append: k and v must both be float32 or bfloat16")
     if k.device != codes.device or v.device != codes.device:
         raise ValueError("kv_append: k and v must be on the cache's device")
-    if k.stride(2) != 1:
+    tokens, _, head_dim = shape
+    kt, kh, kd = k.stride()
+    vt, vh, vd = v.stride()
+    if kd != 1:
         k = k.contiguous()
-    if v.stride(2) != 1:
+        kt, kh, _ = k.stride()
+    if vd != 1:
         v = v.contiguous()
-    tokens, _, head_dim = k.shape
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
+        vt, vh, _ = v.stride()
     ev = _lib.prof_start(k)
     _lib.check(_lib.lib().rt_kv_append(
         codes.data_ptr(), scales.data_ptr(), pages, heads, page_size, width, page_table.data_ptr(),
-        page_table.shape[1], kv_lens.data_ptr(), cu_tokens.data_ptr(), kv_lens.numel(), tokens,
-        k.data_ptr(), v.data_ptr(), _lib.dtype_code(k), head_dim, kt, kh, vt, vh,
+        per_seq, kv_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens, k.data_ptr(), v.data_ptr(), _lib.dtype_code(k), head_dim, kt, kh, vt, vh,
         _lib.stream_of(codes)))
-    _lib.prof_stop(ev, "kv_append", k, 0.0, 2 * k.numel() * (k.element_size() + 1))
+    if ev is not None:
+        _lib.prof_stop(ev, "kv_append", k, 0.0, 2 * k.numel() * (k.element_size() + 1))
 
 
 def kv_read(codes: Tensor, scales: Tensor, page_table: Tensor, starts: Tensor, cu_tokens: Tensor,
@@ -102,22 +115,21 @@ def kv_read(codes: Tensor, scales: Tensor, page_table: Tensor, starts: Tensor, c
             ) -> tuple[Tensor, Tensor]:
     """(k, v) [tokens, kv_heads, head_dim]: the values of the cache at positions starts[s] + i of
     each sequence, row cu_tokens[s] + i; code · scale, rounded once to dtype."""
-    _check_cache(codes, scales, "kv_read")
-    _check_batch(page_table, starts, cu_tokens, "kv_read")
-    pages, _, heads, page_size, width = codes.shape
+    pages, _, heads, page_size, width = _check_cache(codes, scales, "kv_read")
+    seqs, per_seq = _check_batch(page_table, starts, cu_tokens, "kv_read")
     head_dim = width if head_dim is None else head_dim
     if tokens < 0 or not 0 < head_dim <= width:
         raise ValueError("kv_read: tokens must be >= 0 and head_dim in [1, stored width]")
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("kv_read: dtype must be float32 or bfloat16")
     out = torch.empty((2, tokens, heads, head_dim), device=codes.device, dtype=dtype)
-    k, v = out[0], out[1]
+    k, v = out.unbind(0)
     ev = _lib.prof_start(out)
     _lib.check(_lib.lib().rt_kv_read(
         codes.data_ptr(), scales.data_ptr(), pages, heads, page_size, width, page_table.data_ptr(),
-        page_table.shape[1], starts.data_ptr(), cu_tokens.data_ptr(), starts.numel(), tokens, head_dim,
-        k.data_ptr(), v.data_ptr(), _lib.dtype_code(out), _lib.stream_of(codes)))
-    _lib.prof_stop(ev, "kv_read", out, 0.0, out.numel() * (out.element_size() + 1))
+        per_seq, starts.data_ptr(), cu_tokens.data_ptr(), seqs, tokens, head_dim, k.data_ptr(), v.data_ptr(), _lib.dtype_code(out), _lib.stream_of(codes)))
+    if ev is not None:
+        _lib.prof_stop(ev, "kv_read", out, 0.0, out.numel() * (out.element_size() + 1))
     return k, v
 
 
@@ -126,7 +138,7 @@ def kv_copy_pages(codes: Tensor, scales: Tensor, src: Tensor, dst: Tensor, *,
     """Copies pages src[i] to dst[i] (int32 on the device) in every layer of codes [layers, pages, ...]
     and scales, in one launch.  page_table, when given, has every entry equal to src[i] replaced by
     dst[i]: the pages are moved.  No page may be source and destination, or destination twice."""
-    _check_cache(codes, scales, "kv_copy_pages", ndim=6)
+    layers, pages, _, heads, page_size, width = _check_cache(codes, scales, "kv_copy_pages", ndim=6)
     if src.dtype is not torch.int32 or dst.dtype is not torch.int32 or (
             page_table is not None and page_table.dtype is not torch.int32):
         raise TypeError("kv_copy_pages: src, dst and page_table must be int32")
@@ -137,14 +149,14 @@ def kv_copy_pages(codes: Tensor, scales: Tensor, src: Tensor, dst: Tensor, *,
     if not (src.is_contiguous() and dst.is_contiguous()
             and (page_table is None or page_table.is_contiguous())):
         raise ValueError("kv_copy_pages: src, dst and page_table must be contiguous")
-    layers, pages, _, heads, page_size, width = codes.shape
     ev = _lib.prof_start(codes)
     _lib.check(_lib.lib().rt_kv_copy_pages(
         codes.data_ptr(), scales.data_ptr(), layers, pages, heads, page_size, width, src.data_ptr(),
         dst.data_ptr(), src.numel(), _lib.ptr(page_table),
         0 if page_table is None else page_table.numel(), _lib.stream_of(codes)))
-    _lib.prof_stop(ev, "kv_copy_pages", codes, 0.0,
-                   2 * layers * src.numel() * 2 * heads * page_size * (width + 4 / QUANT_BLOCK))
+    if ev is not None:
+        _lib.prof_stop(ev, "kv_copy_pages", codes, 0.0,
+                       2 * layers * src.numel() * 2 * heads * page_size * (width + 4 / QUANT_BLOCK))
 
 
 def kv_attention(q: Tensor, codes: Tensor, scales: Tensor, page_table: Tensor, kv_lens: Tensor,
@@ -156,41 +168,44 @@ def kv_attention(q: Tensor, codes: Tensor, scales: Tensor, page_table: Tensor, k
     Query head h reads key/value head h // (heads / kv_heads).  softmax_scale defaults to
     1 / sqrt(head_dim).  A row that sees no key (or belongs to no sequence) gives zeros.  `out`, when
     given, has q's shape and dtype and a unit innermost stride."""
-    _check_cache(codes, scales, "kv_attention")
-    _check_batch(page_table, kv_lens, cu_tokens, "kv_attention")
-    pages, _, kv_heads, page_size, width = codes.shape
-    if q.dim() != 3 or q.shape[2] > width or q.shape[1] % kv_heads != 0 or q.shape[1] == 0:
+    pages, _, kv_heads, page_size, width = _check_cache(codes, scales, "kv_attention")
+    seqs, per_seq = _check_batch(page_table, kv_lens, cu_tokens, "kv_attention")
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if len(shape) != 3 or shape[2] > width or shape[1] % kv_heads != 0 or shape[1] == 0:
         raise ValueError("kv_attention: q must be [tokens, heads, head_dim] with heads a multiple of "
                          "the cache's heads")
-    if q.dtype not in (torch.float32, torch.bfloat16):
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise TypeError("kv_attention: q must be float32 or bfloat16")
-    if q.device != codes.device:
+    if device != codes.device:
         raise ValueError("kv_attention: q must be on the cache's device")
-    if q.stride(2) != 1:
+    tokens, heads, head_dim = shape
+    qt, qh, qd = q.stride()
+    if qd != 1:
         q = q.contiguous()
-    tokens, heads, head_dim = q.shape
+        qt, qh, _ = q.stride()
     if out is None:
-        out = torch.empty((tokens, heads, head_dim), device=q.device, dtype=q.dtype)
-    elif (out.shape != q.shape or out.dtype is not q.dtype or out.stride(2) != 1
-          or out.device != q.device):
-        raise ValueError("kv_attention: out must have q's shape, dtype and device and a unit last stride")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ot, oh = heads * head_dim, head_dim
+    else:
+        if (out.shape != shape or out.dtype is not dtype or out.stride(2) != 1
+                or out.device != device):
+            raise ValueError("kv_attention: out must have q's shape, dtype and device and a unit last "
+                             "stride")
+        ot, oh, _ = out.stride()
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(head_dim)
-    lib = _lib.lib()
-    seqs = kv_lens.numel()
-    nbytes = lib.rt_kv_attention_workspace_bytes(seqs, tokens, heads, kv_heads, width)
+    nbytes = _attention_workspace(seqs, tokens, heads, kv_heads, width, device.index)
     # allocated per call: the caching allocator keeps calls on different streams apart
-    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
-    qt, qh, _ = q.stride()
-    ot, oh, _ = out.stride()
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
     ev = _lib.prof_start(q)
-    _lib.check(lib.rt_kv_attention(
-        q.data_ptr(), _lib.dtype_code(q), qt, qh, heads, head_dim, codes.data_ptr(),
-        scales.data_ptr(), pages, kv_heads, page_size, width, page_table.data_ptr(),
-        page_table.shape[1], kv_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens,
-        softmax_scale, out.data_ptr(), ot, oh, _lib.ptr(ws), nbytes, _lib.stream_of(q)))
-    # the lengths are on the device: only the rows' own bytes are counted here
-    _lib.prof_stop(ev, "kv_attention", q, 0.0, 2 * q.numel() * q.element_size())
+    _lib.check(_lib.lib().rt_kv_attention(
+        q.data_ptr(), _lib.F32 if dtype is torch.float32 else _lib.BF16, qt, qh, heads, head_dim,
+        codes.data_ptr(), scales.data_ptr(), pages, kv_heads, page_size, width, page_table.data_ptr(),
+        per_seq, kv_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens, softmax_scale, out.data_ptr(),
+        ot, oh, ws.data_ptr(), nbytes, _lib.stream_of(q)))
+    if ev is not None:
+        # the lengths are on the device: only the rows' own bytes are counted here
+        _lib.prof_stop(ev, "kv_attention", q, 0.0, 2 * q.numel() * q.element_size())
     return out
 
 
