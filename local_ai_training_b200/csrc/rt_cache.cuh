@@ -15,6 +15,35 @@ namespace rt {
 
 constexpr int KV_BLOCK = 16;  // tokens that share a scale
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 struct KvCache {
   int8_t *codes;
   float *scales;
@@ -74,17 +103,26 @@ __device__ __forceinline__ int64_t kv_page(const KvCache &c, const KvBatch &b, i
   const int32_t p = kv_entry(c, b, s, blk, INT32_MAX);
   return kv_page_ok(c, p, blk, INT32_MAX) ? p : -1;
 }
-// The sequence whose rows hold row t (cu[s] <= t < cu[s + 1]), or -1.
-__device__ __forceinline__ int64_t kv_seq_of(const int32_t *cu, int64_t n_seqs, int64_t t) {
-  int64_t lo = 0, hi = n_seqs;  // first s with cu[s + 1] > t
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid + 1) > t)
-      hi = mid;
-    else
-      lo = mid + 1;
+// Last s in [0, n_seqs) with key(s) <= x for a non-decreasing key and key(0) <= x (else 0), by a whole warp:
+// each round of 32 probes is one trip to memory (two for 1024 sequences).
+template <typename K>
+__device__ __forceinline__ int64_t kv_warp_search(int64_t n_seqs, int64_t x, const K &key) {
+  int64_t lo = 0, span = n_seqs;
+  while (span > 1) {
+    const int64_t step = (span + 31) >> 5, at = (threadIdx.x & 31) * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, at < span && key(lo + at) <= x);
+    const int64_t skip = max(__popc(below) - 1, 0) * step;
+    lo += skip;
+    span = min(step, span - skip);
   }
-  return lo < n_seqs && __ldg(cu + lo) <= t ? lo : -1;
+  return lo;
+}
+// The sequence whose rows hold row t (cu[s] <= t < cu[s + 1]), or -1; by a whole warp.  (Of sequences that
+// begin at the same row the last is the one that may hold it.)
+__device__ __forceinline__ int64_t kv_seq_of(const int32_t *cu, int64_t n_seqs, int64_t t) {
+  if (n_seqs == 0) return -1;
+  const int64_t s = kv_warp_search(n_seqs, t, [&](int64_t i) { return static_cast<int64_t>(__ldg(cu + i)); });
+  return __ldg(cu + s) <= t && t < __ldg(cu + s + 1) ? s : -1;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -102,39 +140,30 @@ struct KvNew {
   int head_dim;
 };
 
-// What one warp appends: rows [p0, p1) of a block are new (rows before p0 were held).
+// What one warp appends: rows [p0, p1) of a block are new (rows before p0 were held); then the same of
+// the block's next (K|V, head) pieces, every `stride` of them.
 struct KvPiece {
-  int8_t *dst;   // the block's codes
-  float *scale;
-  int64_t row;   // the call's row at the block's row 0 (before the first new one: not read)
-  int part, head, p0, p1;
+  int64_t page;
+  int64_t row;  // the call's row at the block's row 0 (before the first new one: not read)
+  int in_page, p0, p1;
+  int piece, stride;  // K's heads, then V's
 };
 __device__ __forceinline__ bool kv_append_piece(const KvCache &c, const KvBatch &b, int slots, KvPiece &x) {
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int per = 2 * c.kv_heads;
-  const int slot = static_cast<int>(w / per), rest = static_cast<int>(w % per);
-  if (slot >= slots) return false;
-  int64_t lo = 0, hi = b.n_seqs;  // last s whose first slot is <= slot
-  while (lo + 1 < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if ((max(__ldg(b.cu + mid), 0) >> 4) + 2 * mid <= slot)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  const KvSeq q = kv_seq(b, c.page_size, lo);
+  const int slot = blockIdx.x;
+  const int64_t s = kv_warp_search(b.n_seqs, slot, [&](int64_t i) {
+    return static_cast<int64_t>(max(__ldg(b.cu + i), 0) >> 4) + 2 * i;
+  });
+  const KvSeq q = kv_seq(b, c.page_size, s);
   if (q.n == 0) return false;
-  const int blk = (max(q.start, 0) >> 4) + slot - ((q.c0 >> 4) + 2 * static_cast<int>(lo));
+  const int blk = (max(q.start, 0) >> 4) + slot - ((q.c0 >> 4) + 2 * static_cast<int>(s));
   if (blk * KV_BLOCK >= q.len || blk < 0) return false;
-  const int64_t page = kv_page(c, b, lo, blk);
-  if (page < 0) return false;
-  const int in_page = blk & ((c.page_size >> 4) - 1);
-  x.part = rest >= c.kv_heads, x.head = rest - x.part * c.kv_heads;
-  x.dst = c.block(page, x.part, x.head, in_page);
-  x.scale = c.scale(page, x.part, x.head, in_page);
+  x.page = kv_page(c, b, s, blk);
+  if (x.page < 0) return false;
+  x.in_page = blk & ((c.page_size >> 4) - 1);
   x.p0 = max(q.start - blk * KV_BLOCK, 0);
   x.p1 = min(q.len - blk * KV_BLOCK, KV_BLOCK);
   x.row = q.c0 + static_cast<int64_t>(blk) * KV_BLOCK - q.start;
+  x.piece = blockIdx.y * 8 + (threadIdx.x >> 5), x.stride = gridDim.y * 8;
   return true;
 }
 __device__ __forceinline__ int8_t kv_code(float v, float s) {
@@ -150,41 +179,47 @@ __global__ void __launch_bounds__(256) kv_append_any_kernel(KvCache c, KvBatch b
   const int lane = threadIdx.x & 31;
   KvPiece p;
   if (!kv_append_piece(c, b, slots, p)) return;
-  const int64_t st = p.part == 0 ? x.k_token : x.v_token, sh = p.part == 0 ? x.k_head : x.v_head;
-  const T *src = static_cast<const T *>(p.part == 0 ? x.k : x.v) + p.row * st + p.head * sh;
-  float amax = 0.0f;
-  bool odd = false;
-  for (int r = p.p0; r < p.p1; ++r)
-    for (int d = lane; d < x.head_dim; d += 32) {
-      const float a = fabsf(load_as_float(src + r * st + d));
-      if (a <= FLT_MAX)
-        amax = fmaxf(amax, a);
-      else
-        odd = true;
+  for (; p.piece < 2 * c.kv_heads; p.piece += p.stride) {
+    const int part = p.piece >= c.kv_heads, head = p.piece - part * c.kv_heads;
+    int8_t *dst = c.block(p.page, part, head, p.in_page);
+    float *scale = c.scale(p.page, part, head, p.in_page);
+    const int64_t st = part == 0 ? x.k_token : x.v_token, sh = part == 0 ? x.k_head : x.v_head;
+    const T *src = static_cast<const T *>(part == 0 ? x.k : x.v) + p.row * st + head * sh;
+    float amax = 0.0f;
+    bool odd = false;
+    for (int r = p.p0; r < p.p1; ++r)
+      for (int d = lane; d < x.head_dim; d += 32) {
+        const float a = fabsf(load_as_float(src + r * st + d));
+        if (a <= FLT_MAX)
+          amax = fmaxf(amax, a);
+        else
+          odd = true;
+      }
+    amax = warp_max(amax);
+    if (odd) raise_status(RT_STATUS_NONFINITE_KV);
+    const float old = p.p0 > 0 ? *scale : 0.0f;
+    const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
+    if (p.p0 > 0 && s > old) {
+      const float ratio = __fdiv_rn(old, s);
+      for (int i = lane; i < p.p0 * c.dim; i += 32)
+        dst[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(dst[i]), ratio)));
     }
-  amax = warp_max(amax);
-  if (odd) raise_status(RT_STATUS_NONFINITE_KV);
-  const float old = p.p0 > 0 ? *p.scale : 0.0f;
-  const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
-  if (p.p0 > 0 && s > old) {
-    const float ratio = __fdiv_rn(old, s);
-    for (int i = lane; i < p.p0 * c.dim; i += 32)
-      p.dst[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(p.dst[i]), ratio)));
+    for (int r = p.p0; r < p.p1; ++r)
+      for (int d = lane; d < c.dim; d += 32)
+        dst[r * c.dim + d] = d < x.head_dim ? kv_code(load_as_float(src + r * st + d), s) : 0;
+    __syncwarp();
+    if (lane == 0) *scale = s;
   }
-  for (int r = p.p0; r < p.p1; ++r)
-    for (int d = lane; d < c.dim; d += 32)
-      p.dst[r * c.dim + d] = d < x.head_dim ? kv_code(load_as_float(src + r * st + d), s) : 0;
-  __syncwarp();
-  if (lane == 0) *p.scale = s;
 }
 
 // Rows of whole stored width in 16-byte accesses: a block's new rows are read once and stay in registers.
-// Bound by HBM (the element's bytes read, one written); the division is replaced by a product with
-// 1 / s where that rounds to the same code, which it does unless x / s lies within 2^-15 of the middle
-// between two codes (both are within 127 · 1.5 · 2^-23 of the exact quotient); those elements, a few in
-// 10^5, are divided.
+// Bound by HBM (the element's bytes read, one written) with the arithmetic close behind, so x / s is taken
+// by Markstein's theorem (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990): with y = RN(1 / s) and q = RN(x y), RN(q + RN(x - q s) y) is RN(x / s).  (Bounding
+// the product x y instead and dividing near the middle between two codes took 20 % of the accesses of
+// bf16 rows through the division: few-bit operands meet the middle often.)
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
+__global__ void __launch_bounds__(256, sizeof(T) * D <= 256 ? 3 : 1) kv_append_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
   constexpr int E = 16 / sizeof(T);          // elements of an access
   constexpr int LPR = D / E < 32 ? D / E : 32;  // lanes of a row
   constexpr int RPP = 32 / LPR;              // rows of a pass
@@ -195,102 +230,123 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, KvBatch b, Kv
   const int lane = threadIdx.x & 31;
   KvPiece p;
   if (!kv_append_piece(c, b, slots, p)) return;
-  const int64_t st = p.part == 0 ? x.k_token : x.v_token, sh = p.part == 0 ? x.k_head : x.v_head;
   const int r0 = lane / LPR, col = lane % LPR * E;
-  const T *src = static_cast<const T *>(p.part == 0 ? x.k : x.v) + p.row * st + p.head * sh + col;
-  uint4 v[PASSES * CH];
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int r = r0 + i * RPP;
-      v[i * CH + k] = make_uint4(0, 0, 0, 0);
-      if (r >= p.p0 && r < p.p1)
-        v[i * CH + k] = __ldcs(reinterpret_cast<const uint4 *>(src + r * st + k * LPR * E));
-    }
-  const float old = p.p0 > 0 ? *p.scale : 0.0f;
-  const auto element = [&](const uint4 &u, int e) {
+  const auto element = [](const uint4 &u, int e) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
     return __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
   };
-  uint32_t top = 0;  // |x| as bits: order and all, with infinity and NaN above every number
+#pragma unroll 1
+  for (; p.piece < 2 * c.kv_heads; p.piece += p.stride) {
+    const int part = p.piece >= c.kv_heads, head = p.piece - part * c.kv_heads;
+    const int64_t st = part == 0 ? x.k_token : x.v_token, sh = part == 0 ? x.k_head : x.v_head;
+    const T *src = static_cast<const T *>(part == 0 ? x.k : x.v) + (p.row + r0) * st + head * sh + col;
+    uint4 v[PASSES * CH];
 #pragma unroll
-  for (int i = 0; i < PASSES * CH; ++i)
+    for (int i = 0; i < PASSES; ++i)
 #pragma unroll
-    for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(element(v[i], e)) & 0x7FFFFFFFu);
-  float amax = __uint_as_float(top);
-  bool odd = top >= 0x7F800000u;
-  if (__any_sync(0xffffffffu, odd)) {
-    if (odd) raise_status(RT_STATUS_NONFINITE_KV);
-    odd = true;
-    amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PASSES * CH; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float a = fabsf(element(v[i], e));
-        if (a <= FLT_MAX) amax = fmaxf(amax, a);
+      for (int k = 0; k < CH; ++k) {
+        const int r = r0 + i * RPP;
+        v[i * CH + k] = make_uint4(0, 0, 0, 0);
+        if (r >= p.p0 && r < p.p1)
+          v[i * CH + k] = __ldcs(reinterpret_cast<const uint4 *>(src + i * RPP * st + k * LPR * E));
       }
-  }
-  amax = warp_max(amax);
-  const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
-  if (p.p0 > 0 && s > old) {
-    const float ratio = __fdiv_rn(old, s);
-    for (int i = lane; i < p.p0 * (D / 4); i += 32) {
-      char4 *at = reinterpret_cast<char4 *>(p.dst) + i;
-      char4 q = *at;
-      q.x = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.x), ratio)));
-      q.y = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.y), ratio)));
-      q.z = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.z), ratio)));
-      q.w = static_cast<signed char>(__float2int_rn(__fmul_rn(static_cast<float>(q.w), ratio)));
-      *at = q;
+    int8_t *dst = c.block(p.page, part, head, p.in_page);
+    float *scale = c.scale(p.page, part, head, p.in_page);
+    const float old = p.p0 > 0 ? *scale : 0.0f;
+    // |x| as bits: order and all, with infinity and NaN above every number (bf16: two 16-bit halves)
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < PASSES * CH; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4)
+          top = max(top, w[e] & 0x7FFFFFFFu);
+        else
+          top = __vmaxu2(top, w[e] & 0x7FFF7FFFu);
+      }
     }
-  }
-  const float inv = __fdiv_rn(1.0f, s);
-  const bool divide = odd || s > 1e37f;  // (1 / s must be a normal number)
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i)
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const uint4 u = v[i * CH + k];
-      uint32_t code[E / 4];
-      float off = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        uint32_t q[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // 1.5 · 2^23 + rint(x / s): the code is the low byte
-          const float y = __fmaf_rn(element(u, e + j), inv, 12582912.0f);
-          off = fmaxf(off, fabsf(__fmaf_rn(element(u, e + j), inv, 12582912.0f - y)));
-          q[j] = __float_as_uint(y);
+    if constexpr (sizeof(T) == 2) top = max(top & 0xFFFF0000u, top << 16);
+    float amax = __uint_as_float(top);
+    const bool odd = __any_sync(0xffffffffu, top >= 0x7F800000u);
+    if (odd) {
+      if (top >= 0x7F800000u) raise_status(RT_STATUS_NONFINITE_KV);
+      amax = 0.0f;
+#pragma unroll 1
+      for (int r = max(p.p0, r0); r < p.p1; ++r) {
+        if ((r - r0) % RPP != 0) continue;
+#pragma unroll 1
+        for (int e = 0; e < CH * E; ++e) {
+          const float a = fabsf(load_as_float(src + (r - r0) * st + e / E * (LPR * E) + e % E));
+          if (a <= FLT_MAX) amax = fmaxf(amax, a);
         }
-        code[e / 4] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
       }
-      if (divide || off > 0.5f - 3.0517578125e-5f) {
+    }
+    amax = warp_max(amax);
+    const float s = fmaxf(fmaxf(old, __fdiv_rn(amax, 127.0f)), FLT_MIN);
+    if (p.p0 > 0 && s > old) {
+      const float ratio = __fdiv_rn(old, s);
+#pragma unroll 2
+      for (int i = lane; i < p.p0 * (D / 16); i += 32) {
+        uint4 *at = reinterpret_cast<uint4 *>(dst) + i;
+        const uint4 u = *at;
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t q[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            q[j] = __float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[e] >> 8 * j)), ratio));
+          w[e] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        }
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    const float inv = __fdiv_rn(1.0f, s);
+    const float2 inv2 = make_float2(inv, inv), neg_s = make_float2(-s, -s);
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i)
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const uint4 u = v[i * CH + k];
+        uint32_t code[E / 4];
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-          uint32_t w = 0;
-#pragma unroll 1
-          for (int j = 3; j >= 0; --j) {
-            const float f = j == 0 ? element(u, e) : j == 1 ? element(u, e + 1) : j == 2 ? element(u, e + 2) : element(u, e + 3);
-            w = w << 8 | static_cast<uint8_t>(kv_code(f, s));
+          uint32_t q[4];
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const float2 f = make_float2(element(u, e + j), element(u, e + j + 1));
+            float2 y = mul2(f, inv2);
+            y = fma2(fma2(y, neg_s, f), inv2, y);
+            // 1.5 · 2^23 + rint(x / s): the code is the low byte
+            y = add2(y, make_float2(12582912.0f, 12582912.0f));
+            q[j] = __float_as_uint(y.x), q[j + 1] = __float_as_uint(y.y);
           }
-          code[e / 4] = w;
+          code[e / 4] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        }
+        const int r = r0 + i * RPP;
+        if (r >= p.p0 && r < p.p1) {
+          uint32_t *at = reinterpret_cast<uint32_t *>(dst + r * D + k * LPR * E + col);
+          if constexpr (E == 8)
+            *reinterpret_cast<uint2 *>(at) = make_uint2(code[0], code[1]);
+          else
+            *at = code[0];
         }
       }
-      const int r = r0 + i * RPP;
-      if (r >= p.p0 && r < p.p1) {
-        uint32_t *dst = reinterpret_cast<uint32_t *>(p.dst + r * D + k * LPR * E + col);
-        if constexpr (E == 8)
-          *reinterpret_cast<uint2 *>(dst) = make_uint2(code[0], code[1]);
-        else
-          *dst = code[0];
+    if (odd || s > 1e37f || s < 1e-30f) {  // infinities and NaN; 1 / s or the remainder not a normal number
+#pragma unroll 1
+      for (int i = 0; i < PASSES * CH; ++i) {
+        const int r = r0 + i / CH * RPP, at = i % CH * LPR * E;
+        if (r < p.p0 || r >= p.p1) continue;
+#pragma unroll 1
+        for (int e = 0; e < E; ++e)
+          dst[r * D + at + col + e] = kv_code(load_as_float(src + (r - r0) * st + at + e), s);
       }
     }
-  __syncwarp();
-  if (lane == 0) *p.scale = s;
+    __syncwarp();
+    if (lane == 0) *scale = s;
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -315,13 +371,14 @@ __global__ void __launch_bounds__(256)
   __shared__ int64_t sm_page[KR_ROWS];
   __shared__ int sm_pos[KR_ROWS];
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * KR_ROWS;
-  if (threadIdx.x < KR_ROWS && t0 + threadIdx.x < b.n_tokens) {
-    const int64_t t = t0 + threadIdx.x, s = kv_seq_of(b.cu, b.n_seqs, t);
+  const int warp = threadIdx.x >> 5;
+  if (warp < KR_ROWS && t0 + warp < b.n_tokens) {
+    const int64_t t = t0 + warp, s = kv_seq_of(b.cu, b.n_seqs, t);
     const int64_t pos = s < 0 ? -1 : __ldg(b.kv_lens + s) + t - __ldg(b.cu + s);
     const bool in = pos >= 0 && pos < b.pages_per_seq * c.page_size;
     if (s >= 0 && !in) raise_status(RT_STATUS_INDEX_RANGE);
-    sm_page[threadIdx.x] = in ? kv_page(c, b, s, static_cast<int>(pos >> 4)) : -1;
-    sm_pos[threadIdx.x] = static_cast<int>(pos);
+    sm_page[warp] = in ? kv_page(c, b, s, static_cast<int>(pos >> 4)) : -1;
+    sm_pos[warp] = static_cast<int>(pos);
   }
   __syncthreads();
   const int rows = static_cast<int>(min(static_cast<int64_t>(KR_ROWS), b.n_tokens - t0));
@@ -378,12 +435,14 @@ __global__ void __launch_bounds__(256)
 // ------------------------------------------------------------------------------------------
 // Page copies over all layers, and the page table's entries rewritten from src to dst.
 // ------------------------------------------------------------------------------------------
+// Bound by HBM (a byte read and one written): CTAs of 16 KB, so that a few pages use the whole GPU too.
+constexpr int KC_CHUNK = 4 * 256;  // 16-byte accesses of a CTA
 struct KvCopy {
   int8_t *codes;
   float *scales;
   int64_t layers, n_pages, page_bytes, page_scales;
   const int32_t *src, *dst;
-  int n;
+  int n, chunks;
   int32_t *table;
   int64_t entries;
 };
@@ -402,7 +461,8 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvCopy a, int copy_blocks)
       }
     return;
   }
-  const int64_t pair = blockIdx.x % a.n, layer = blockIdx.x / a.n;
+  const int chunk = blockIdx.x % a.chunks;
+  const int64_t which = blockIdx.x / a.chunks, pair = which % a.n, layer = which / a.n;
   const int32_t s = __ldg(a.src + pair), d = __ldg(a.dst + pair);
   if (s < 0 || s >= a.n_pages || d < 0 || d >= a.n_pages) {
     raise_status(RT_STATUS_INDEX_RANGE);
@@ -410,7 +470,18 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(KvCopy a, int copy_blocks)
   }
   const int4 *from = reinterpret_cast<const int4 *>(a.codes + (layer * a.n_pages + s) * a.page_bytes);
   int4 *to = reinterpret_cast<int4 *>(a.codes + (layer * a.n_pages + d) * a.page_bytes);
-  for (int64_t i = threadIdx.x; i < a.page_bytes / 16; i += blockDim.x) to[i] = from[i];
+  // four 16-byte accesses of a thread under way at a time
+  const int64_t end = min(static_cast<int64_t>(chunk + 1) * KC_CHUNK, a.page_bytes / 16);
+  for (int64_t i = static_cast<int64_t>(chunk) * KC_CHUNK + threadIdx.x; i < end; i += KC_CHUNK) {
+    int4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * 256 < end) v[k] = __ldcs(from + i + k * 256);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * 256 < end) __stcs(to + i + k * 256, v[k]);
+  }
+  if (chunk != 0) return;
   const float *sf = a.scales + (layer * a.n_pages + s) * a.page_scales;
   float *st = a.scales + (layer * a.n_pages + d) * a.page_scales;
   for (int64_t i = threadIdx.x; i < a.page_scales; i += blockDim.x) st[i] = sf[i];
@@ -477,8 +548,9 @@ extern "C" int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t
   const KvNew x{k, v, k_stride_token, k_stride_head, v_stride_token, v_stride_head,
                 static_cast<int>(head_dim)};
   const int64_t slots = n_tokens / KV_BLOCK + 2 * n_seqs;
-  const int64_t grid = (slots * 2 * kv_heads + 7) / 8;
-  if (grid > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "kv_append: batch too large");
+  // A warp per (slot, K|V, head); four pieces a warp, one after the other, hid less latency.
+  const int64_t pieces = (2 * kv_heads + 7) / 8;
+  const dim3 grid(static_cast<unsigned>(slots), static_cast<unsigned>(pieces));
   const int es = dtype == RT_F32 ? 4 : 2;
   const bool vec = head_dim == padded_dim && aligned16(k) && aligned16(v) && k_stride_token * es % 16 == 0 &&
                    k_stride_head * es % 16 == 0 && v_stride_token * es % 16 == 0 &&
@@ -486,7 +558,7 @@ extern "C" int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t
   // (an fp32 block of width 256 does not fit a warp's registers)
   const auto kernel = [&](auto *any, auto *d32, auto *d64, auto *d128, auto *d256) {
     auto *f = !vec ? any : padded_dim == 32 ? d32 : padded_dim == 64 ? d64 : padded_dim == 128 ? d128 : d256;
-    launch_k(f, static_cast<unsigned>(grid), 256, 0, as_stream(stream), c, b, x, static_cast<int>(slots));
+    launch_k(f, grid, 256, 0, as_stream(stream), c, b, x, static_cast<int>(slots));
   };
   if (dtype == RT_F32)
     kernel(kv_append_any_kernel<float>, kv_append_kernel<float, 32>, kv_append_kernel<float, 64>,
@@ -541,11 +613,12 @@ extern "C" int rt_kv_copy_pages(void *codes, float *scales, int64_t layers, int6
   if (n == 0) return RT_OK;
   if (src == nullptr || dst == nullptr || (page_table == nullptr && table_entries > 0))
     return fail(RT_ERR_INVALID_ARGUMENT, "kv_copy_pages: null pointer");
-  const int64_t blocks = n * layers, table_blocks = (table_entries + 255) / 256;
+  const int64_t chunks = (c.page_bytes() / 16 + KC_CHUNK - 1) / KC_CHUNK;
+  const int64_t blocks = n * layers * chunks, table_blocks = (table_entries + 255) / 256;
   if (n > n_pages || blocks + table_blocks > INT32_MAX)
     return fail(RT_ERR_UNSUPPORTED, "kv_copy_pages: more pairs than pages");
   KvCopy a{c.codes, c.scales, layers, n_pages, c.page_bytes(),
-           2 * kv_heads * (page_size / KV_BLOCK), src, dst, static_cast<int>(n), page_table,
+           2 * kv_heads * (page_size / KV_BLOCK), src, dst, static_cast<int>(n), static_cast<int>(chunks), page_table,
            table_entries};
   launch_k(kv_copy_kernel, static_cast<unsigned>(blocks + table_blocks), 256, 0, as_stream(stream),
            a, static_cast<int>(blocks));

@@ -218,6 +218,7 @@ class CacheBatch:
     cu_tokens: Tensor
     positions: Tensor  # int64 [tokens]: position of each new row in its sequence
     n_tokens: int
+    max_length: int  # of the sequences, with their newest tokens
 
 
 class PagedKVCache:
@@ -371,7 +372,8 @@ class PagedKVCache:
         b = a + len(seqs)
         c = b + len(cu)
         return CacheBatch(packed[:a].view(len(seqs), width), packed[a:b], packed[b:c],
-                          packed[c:].long(), cu[-1])
+                          packed[c:].long(), cu[-1],
+                          max([self._lens[s] for s in seqs], default=0))
 
     # ------------------------------------------------------------------ operators
     def append(self, layer: int, batch: CacheBatch, k: Tensor, v: Tensor) -> None:

@@ -4,7 +4,8 @@ Same configuration fields, module tree, parameter names and initialisation order
 (so seeded models and state_dicts match); the int8 path routes through the fused producers and
 the ratchet layers of this package.  The lm_head and the token cross-entropy run as fused CUDA
 kernels of this library (cross_entropy.py); attention (SDPA), the embedding lookup and the
-optimizer stay PyTorch ops.
+optimizer stay PyTorch ops.  `forward_cached` runs the newest tokens of sequences over a paged int8
+key/value cache (kv_cache.py) for generation (generate.py).
 """
 
 from __future__ import annotations
@@ -20,6 +21,8 @@ from torch.nn import functional as F
 
 from .int8_fused import (FusedGELUQuantizeFn, FusedRMSNormQuantizeFn, FusedTransposeQuantizeFn,
                          QKVHeadsFn)
+from .int8_matmul import quantize_rows
+from .kv_cache import CacheBatch, PagedKVCache
 from .ratchet import DiscreteRatchetLinear, RatchetEmbedding, RatchetUpdateStats, grad_plan_of
 
 
@@ -114,6 +117,15 @@ def _linear(config: ModelConfig, in_features: int, out_features: int, max_code: 
     )
 
 
+@dataclass(frozen=True)
+class CachedLayer:
+    """A layer's place in a key/value cache and the batch whose newest tokens are computed."""
+
+    cache: PagedKVCache
+    batch: CacheBatch
+    layer: int
+
+
 class CausalSelfAttention(nn.Module):
     def __init__(self, config: ModelConfig, *, max_code: int | None) -> None:
         super().__init__()
@@ -127,15 +139,19 @@ class CausalSelfAttention(nn.Module):
 
     def forward(self, inputs: Tensor, *, inputs_int8: Tensor | None = None,
                 inputs_scale: Tensor | None = None, residual: Tensor | None = None,
-                inputs_dequant: Tensor | None = None) -> Tensor:
+                inputs_dequant: Tensor | None = None, cached: CachedLayer | None = None) -> Tensor:
         """residual (int8 path): returns residual + attention(...), the add in the projection's
-        GEMM epilogue.  inputs_dequant: the producer's bf16 dequantised rows (qkv grad_weight)."""
+        GEMM epilogue.  inputs_dequant: the producer's bf16 dequantised rows (qkv grad_weight).
+        cached (no gradient): the rows are the newest tokens of a batch of sequences; their keys and
+        values are appended to the cache and they attend over it."""
         batch_size, sequence_length, channels = inputs.shape
         if inputs_int8 is not None:
             qkv = self.qkv(inputs, inputs_int8=inputs_int8, inputs_scale=inputs_scale,
                            inputs_dequant=inputs_dequant)
         else:
             qkv = self.qkv(inputs)
+        if cached is not None:
+            return self._attend_cached(qkv, cached, residual)
         plan = grad_plan_of(qkv) if self.fused_grad_quant else None
         if plan is not None:
             # the gradients of the three head views come back as the projection's quantised
@@ -158,6 +174,20 @@ class CausalSelfAttention(nn.Module):
             return self.projection(dummy_joined, inputs_int8=attn_int8, inputs_scale=attn_scale,
                                    residual=residual, inputs_dequant=dq[0] if dq else None)
         joined = attended.transpose(1, 2).contiguous().view(batch_size, sequence_length, channels)
+        out = self.projection(joined)
+        return out if residual is None else residual + out
+
+
+    def _attend_cached(self, qkv: Tensor, cached: CachedLayer, residual: Tensor | None) -> Tensor:
+        rows = qkv.flatten(0, 1)
+        query, key, value = (part.view(rows.shape[0], self.n_head, self.head_size)
+                             for part in rows.chunk(3, dim=-1))
+        cached.cache.append(cached.layer, cached.batch, key, value)
+        # rows are tokens already: the projection's input needs no head transpose
+        joined = cached.cache.attend(cached.layer, cached.batch, query).view(1, rows.shape[0], -1)
+        if getattr(self.projection, "matmul_mode", "fp32") == "int8":
+            int8, scale = quantize_rows(joined[0])
+            return self.projection(joined, inputs_int8=int8, inputs_scale=scale, residual=residual)
         out = self.projection(joined)
         return out if residual is None else residual + out
 
@@ -217,7 +247,7 @@ class TransformerBlock(nn.Module):
         self.fused_grad_quant = config.fused_grad_quant
         self.producer_dequant = config.producer_dequant
 
-    def forward(self, inputs: Tensor) -> Tensor:
+    def forward(self, inputs: Tensor, cached: CachedLayer | None = None) -> Tensor:
         # int8 path with fused residuals: the RMSNorm producer hands x on as the residual, the
         # sublayer's last GEMM adds it in its epilogue, and in backward the residual gradient is
         # added to the RMSNorm input gradient by the same kernel (same values as `x + f(x)`)
@@ -231,16 +261,18 @@ class TransformerBlock(nn.Module):
                     inputs, self.attention_norm.weight, 1e-5, self.dummy_dtype, True, plan,
                     self.producer_dequant)
                 inputs = self.attention(dummy_in, inputs_int8=attn_int8, inputs_scale=attn_scale,
-                                        residual=res, inputs_dequant=dq[0] if dq else None)
+                                        residual=res, inputs_dequant=dq[0] if dq else None,
+                                        cached=cached)
             else:
                 attn_int8, attn_scale, dummy_in, *dq = FusedRMSNormQuantizeFn.apply(
                     inputs, self.attention_norm.weight, 1e-5, self.dummy_dtype, False, None,
                     self.producer_dequant)
                 inputs = inputs + self.attention(dummy_in, inputs_int8=attn_int8,
                                                  inputs_scale=attn_scale,
-                                                 inputs_dequant=dq[0] if dq else None)
+                                                 inputs_dequant=dq[0] if dq else None,
+                                                 cached=cached)
         else:
-            inputs = inputs + self.attention(self.attention_norm(inputs))
+            inputs = inputs + self.attention(self.attention_norm(inputs), cached=cached)
         if getattr(self.feed_forward.expand, "matmul_mode", "fp32") == "int8":
             if fused:
                 plan = grad_plan_of(inputs) if self.fused_grad_quant else None
@@ -314,6 +346,34 @@ class RatchetGPT(nn.Module):
         if targets is not None:
             loss = F.cross_entropy(logits.flatten(0, 1), targets.flatten())
         return logits, loss
+
+    @torch.no_grad()
+    def forward_cached(self, tokens: Tensor, cache: PagedKVCache, batch: CacheBatch, *,
+                       last_only: bool = True) -> Tensor:
+        """Logits of a batch's newest tokens over a key/value cache (generation; evaluation mode).
+
+        tokens [batch.n_tokens] are the newest tokens of the batch's sequences one after the other
+        (`cache.reserve` made the batch for them).  last_only: logits [sequences, vocab] of each
+        sequence's last token (every sequence then needs a newest token); else of every token.
+        With the whole text as newest tokens the values are those of `forward` up to the cache's 8-bit
+        keys and values."""
+        if self.training:
+            raise RuntimeError("forward_cached requires evaluation mode (model.eval())")
+        if tokens.ndim != 1 or tokens.shape[0] != batch.n_tokens:
+            raise ValueError("tokens must be the batch's newest tokens, one after the other")
+        if batch.max_length > self.config.block_size:
+            raise ValueError("token sequence exceeds configured block_size")
+        if (cache.n_layer, cache.n_kv_head, cache.head_dim) != (
+                len(self.blocks), self.config.n_head, self.config.n_embd // self.config.n_head):
+            raise ValueError("the cache's layers, heads and head width must be the model's")
+        hidden = self.token_embedding(tokens) + self.position_encoding[batch.positions]
+        hidden = hidden[None]
+        for layer, block in enumerate(self.blocks):
+            hidden = block(hidden, CachedLayer(cache, batch, layer))
+        hidden = hidden[0]
+        if last_only:
+            hidden = hidden[batch.cu_tokens[1:] - 1]
+        return self.lm_head(self.final_norm(hidden))
 
     def ratchet_layers(self) -> list[DiscreteRatchetLinear]:
         if getattr(self, "_ratchet_layers", None) is None:
