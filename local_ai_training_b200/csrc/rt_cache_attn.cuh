@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
           const int tok = (row0 + r) / a.group, h = w.head * a.group + (row0 + r) % a.group;
           store_from_float(static_cast<T *>(a.out) + (w.q.c0 + static_cast<int64_t>(tok)) * a.o_token +
                                static_cast<int64_t>(h) * a.o_head + d,
-                           den > 0.0f ? __fdividef(sum, den) : 0.0f);
+                           den == 0.0f ? 0.0f : __fdividef(sum, den));
         }
       } else {
         float *dst = a.ws + (static_cast<int64_t>(slot) * RT + r) * (D + 4);
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBat
   const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
   const KvSeq q = kv_seq(bt, c.page_size, mt.x);
   const int row = mt.y * RT + r;
-  if (row >= q.n * a.group) return;
+  if (r >= RT || row >= q.n * a.group) return;
   int last = blockIdx.x + 1;  // the CTA that ended the unit
   for (;; last += 32) {
     const int x = last + lane;
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBat
     }
   }
   den = warp_sum_butterfly(den);
-  const float inv = den > 0.0f ? __fdividef(1.0f, den) : 0.0f;
+  const float inv = den == 0.0f ? 0.0f : __fdividef(1.0f, den);
   T *o = static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(row / a.group)) * a.o_token +
          static_cast<int64_t>(mt.z * a.group + row % a.group) * a.o_head;
 #pragma unroll

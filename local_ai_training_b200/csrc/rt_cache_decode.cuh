@@ -1,0 +1,411 @@
+// rt_cache_decode.cuh — attention of few query rows over the paged int8 cache with heads of 128: the
+// mathematics, the work split and the joining of rt_cache_attn.cuh, with both products on the int8
+// tensor cores (tcgen05 kind::i8).
+//
+// The kernel is to run at the rate at which HBM delivers the codes, some 24 a cycle and SM, so a code is touched by no ALU instruction: TMA brings it from its page into the operand layout
+// that the tensor core reads.  What must then be int8 too are q and the weights, as digits:
+//   q_r = qs (c0 + c1 2^-7 + c2 2^-14 [+ c3 2^-21]),  |c0| <= 127, |c1..| <= 64,  qs = max|q_r| / 127
+//   p_j sv_j / max(sv) 127 = the same, p_j = 2^(t_j - m) <= 1 under the running maximum m
+// Three digits hold 22 bits below the largest value (bf16 q has 8, the weights' output is rounded to 8),
+// four digits all 24 of an fp32 q's largest.  Digits of one row are columns of one product:
+//   S^T [128 keys x N] = K (128 x 128 codes) · Q^T (N rows of digits), N = digits · RT
+//   O^T [128 dims x N] = V^T (the tile as it lies, M-major) · P^T (N rows of digits over the keys)
+// Products and sums are exact (|sum| < 2^21); a thread is a key in S^T and a dim in O^T, so it holds all
+// digits of its rows and joins them in fp32.  O is summed in registers, rescaled as m moves.
+//   warps 0-3  scores -> weights -> digits; sums of O, a tile behind, while the tensor core works
+//   warp 4     TMA: page entries, tiles of 128 keys of K and V, block scales
+//   warp 5     one thread issues the products, the next tile's scores before this one's outputs
+#pragma once
+
+#include "rt_cache_attn.cuh"
+#include "rt_tensormap.cuh"
+
+namespace rt {
+
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Barrier of 128 threads that also ands a flag over them.
+__device__ __forceinline__ bool warpgroup_and(int id, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
+// 16 columns, loaded and waited for.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Exact for |v| < 2^22, without the conversion unit.
+__device__ __forceinline__ float small_int(uint32_t v) {
+  return __int_as_float(static_cast<int>(v) + 0x4B400000) - 12582912.0f;
+}
+
+template <typename T, int RT>
+struct KdShape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int D = 128, KEYS = 128;
+  static constexpr int ND = F32 ? 4 : 3;                  // digits
+  static constexpr int N = (RT * ND + 15) / 16 * 16;      // columns of a product
+  static constexpr int STAGES = RT == 4 ? 3 : 2;
+  static constexpr int TILE = KEYS * D, ROWS = N * 128;   // bytes of a K or V tile, of N rows of digits
+  static constexpr int K_OFF = 0, V_OFF = STAGES * TILE, Q_OFF = 2 * STAGES * TILE;
+  static constexpr int P_OFF = Q_OFF + ROWS, F_OFF = P_OFF + 2 * ROWS;
+  static constexpr int M_OFF = F_OFF + STAGES * 80;       // maxima of the four warps [2][RT][4]
+  static constexpr int QS_OFF = M_OFF + 2 * RT * 16;      // qs of the rows
+  static constexpr int BAR_OFF = QS_OFF + RT * 4;
+  static constexpr int SMEM = BAR_OFF + 256 + 1024;
+  static constexpr int TMEM = N == 16 ? 64 : 256;         // two S and two O tiles of N columns
+  static constexpr int CTAS = 2;                          // per SM
+  static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((128 >> 4) << 24);
+  static constexpr uint32_t IDESC_V = IDESC | (1u << 15);  // V^T: M-major
+  static_assert(2 * SMEM <= 227 * 1024, "two CTAs of an SM");
+};
+struct KdBars {
+  uint64_t full[3], empty[3], s_full[2], p_full[2], o_full[2], q_full;
+  uint32_t tmem;
+  int tiles;  // of the piece
+};
+static_assert(sizeof(KdBars) <= 256, "KdBars");
+struct KdFactors {  // one tile's block factors
+  float k[8];       // sk · softmax scale · log2 e
+  float v[8];       // sv / max(sv) · 127
+  float unit;       // max(sv) / 127
+  uint32_t blocks;  // bit i: block i has a page
+};
+
+// Digits of x in [-127, 127], one per byte of the result, the first lowest.
+template <int ND>
+__device__ __forceinline__ uint32_t digits_of(float x) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    const float a = x + 12582912.0f;  // 1.5 · 2^23 + rint(x)
+    w |= (__float_as_uint(a) & 0xFFu) << (8 * i);
+    x = (x - (a - 12582912.0f)) * 128.0f;  // exact
+  }
+  return w;
+}
+template <int ND, int RT>
+__device__ __forceinline__ float joined(const uint32_t *s, int r) {
+  float v = small_int(s[(ND - 1) * RT + r]);
+#pragma unroll
+  for (int i = ND - 2; i >= 0; --i) v = fmaf(v, 0.0078125f, small_int(s[i * RT + r]));
+  return v;
+}
+
+template <typename T, int RT>
+__global__ void __launch_bounds__(192, 2)
+    kv_decode_kernel(const __grid_constant__ CUtensorMap map, KvCache c, KvBatch bt, KvAttn a, int min_blocks) {
+  using SH = KdShape<T, RT>;
+  using Walk = KvWalk<RT, SH::KEYS>;
+  constexpr int ND = SH::ND, N = SH::N, D = SH::D;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  KdBars *bar = reinterpret_cast<KdBars *>(smem + SH::BAR_OFF);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < SH::STAGES; ++i) mbar_init(&bar->full[i], 1), mbar_init(&bar->empty[i], 1);
+    for (int i = 0; i < 2; ++i)
+      mbar_init(&bar->s_full[i], 1), mbar_init(&bar->p_full[i], 128), mbar_init(&bar->o_full[i], 1);
+    mbar_init(&bar->q_full, 128);
+    fence_barrier_init();
+    tma_prefetch_desc(&map);
+  }
+  if (warp == 5) {
+    tmem_alloc(&bar->tmem, SH::TMEM);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  kv_zero_rest<T>(bt, a);
+  Walk w;
+  const bool busy = kv_walk_start<192>(w, c, bt, a, min_blocks);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();  // the next kernel comes up only now that this one has its tensor memory
+  if (!busy) {
+    if (tid == 0 && min_blocks != 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (warp == 5) tmem_dealloc(bar->tmem, SH::TMEM);
+    return;
+  }
+  const uint32_t tmem = bar->tmem;
+
+  if (warp < 4) {
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp) << 21);
+    float *qs = reinterpret_cast<float *>(smem + SH::QS_OFF);
+    uint32_t n = 0, pieces = 0;  // tiles of the CTA
+    bool ok = true;
+    while (w.left > 0) {
+      const int row0 = w.tile * RT, rows = min(RT, w.q.n * a.group - row0);
+      // ---- q's digits: a warp per row, four dims a lane
+#pragma unroll 1
+      for (int r = warp; r < RT; r += 4) {
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < rows) {
+          int token, sub;
+          kv_row(a, row0 + r, token, sub);
+          const T *qp = static_cast<const T *>(a.q) + (w.q.c0 + static_cast<int64_t>(token)) * a.q_token +
+                        static_cast<int64_t>(w.head * a.group + sub) * a.q_head + lane * 4;
+          if (a.q_vec) {
+            if constexpr (SH::F32) {
+              *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp);
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2 *>(qp);
+              x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+              x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xFFFF0000u);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (lane * 4 + i < a.head_dim) x[i] = load_as_float(qp + i);
+          }
+        }
+        float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= !(fabsf(x[i]) <= FLT_MAX);
+        odd = __any_sync(0xffffffffu, odd);
+        amax = redux_max(amax);
+        // (a row below 2^-100 scores nothing; a row with an infinity or a NaN makes its scores NaN)
+        const float inv = amax > 7.8e-31f ? __fdiv_rn(127.0f, amax) : 0.0f;
+        if (lane == 0) qs[r] = odd ? __int_as_float(0x7FC00000) : __fdiv_rn(amax, 127.0f);
+        uint32_t w4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w4[i] = digits_of<ND>(fminf(fmaxf(x[i] * inv, -127.0f), 127.0f));
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          const int row = i * RT + r;
+          const uint32_t word = (w4[0] >> 8 * i & 0xFFu) | (w4[1] >> 8 * i & 0xFFu) << 8 |
+                                (w4[2] >> 8 * i & 0xFFu) << 16 | (w4[3] >> 8 * i & 0xFFu) << 24;
+          *reinterpret_cast<uint32_t *>(smem + SH::Q_OFF + row * 128 + ((lane * 4) ^ ((row & 7) << 4))) = word;
+        }
+      }
+      if (tid == 0) bar->tiles = w.e - w.b;
+      fence_proxy_async_smem();
+      tc_fence_before();
+      mbar_arrive(&bar->q_full);
+      ok = warpgroup_and(1, ok);  // qs of all rows
+
+      float m[RT], l[RT], acc[RT], f[RT], unit = 0.0f;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) m[r] = -1e30f, l[r] = acc[r] = f[r] = 0.0f;
+      // adds the outputs of tile i, whose weights were under the maximum before f's move
+      const auto add_outputs = [&](uint32_t i) {
+        ok = mbar_wait(&bar->o_full[i & 1], (i >> 1) & 1) && ok;
+        tc_fence_after();
+        uint32_t o[N];
+#pragma unroll
+        for (int x = 0; x < N / 16; ++x)
+          tmem_ld_32x32b_x16(t_lane + 2 * N + (i & 1) * N + x * 16, *reinterpret_cast<uint32_t(*)[16]>(o + x * 16));
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r] = fmaf(acc[r], f[r], joined<ND, RT>(o, r) * unit);
+      };
+#pragma unroll 1
+      for (int j = w.b; j < w.e && ok; ++j, ++n) {
+        const int st = n % SH::STAGES;
+        ok = mbar_wait(&bar->full[st], (n / SH::STAGES) & 1) && mbar_wait(&bar->s_full[n & 1], (n >> 1) & 1);
+        tc_fence_after();
+        const KdFactors *fac = reinterpret_cast<const KdFactors *>(smem + SH::F_OFF + st * 80);
+        const float fk = fac->k[tid >> 4], fv = fac->v[tid >> 4], unit_now = fac->unit;
+        const bool has = fac->blocks >> (tid >> 4) & 1;
+        float t[RT];
+        {
+          uint32_t s[N];
+#pragma unroll
+          for (int x = 0; x < N / 16; ++x)
+            tmem_ld_32x32b_x16(t_lane + (n & 1) * N + x * 16, *reinterpret_cast<uint32_t(*)[16]>(s + x * 16));
+#pragma unroll
+          for (int r = 0; r < RT; ++r) t[r] = joined<ND, RT>(s, r) * (fk * qs[r]);
+        }
+        const int key = j * SH::KEYS + tid;
+        if ((j + 1) * SH::KEYS > w.seen(a, row0 + 1) || fac->blocks != 0xFFu) {  // a key some row does not see
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (!has || key >= w.seen(a, row0 + min(r, rows - 1) + 1)) t[r] = -INFINITY;
+        }
+        float *mx = reinterpret_cast<float *>(smem + SH::M_OFF) + (n & 1) * RT * 4;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float v = redux_max(t[r]);
+          if (lane == r) mx[r * 4 + warp] = v;
+        }
+        ok = warpgroup_and(1, ok);
+        if (!ok) break;
+        uint8_t *pt = smem + SH::P_OFF + (n & 1) * SH::ROWS;
+        float g[RT];  // how far the maxima move
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float4 v = *reinterpret_cast<const float4 *>(mx + r * 4);
+          const float mn = fmaxf(m[r], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+          g[r] = ex2(m[r] - mn);
+          m[r] = mn;
+          const float p = ex2(t[r] - mn);
+          l[r] = fmaf(l[r], g[r], p);
+          const uint32_t dg = digits_of<ND>(p * fv);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const int row = i * RT + r;
+            pt[row * 128 + (tid ^ ((row & 7) << 4))] = static_cast<uint8_t>(dg >> (8 * i));
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&bar->p_full[n & 1]);
+        if (j > w.b) add_outputs(n - 1);
+        unit = unit_now;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) f[r] = g[r];
+      }
+      // ---- the piece's rows: thread = dim
+      if (ok) add_outputs(n - 1);
+      float *red = reinterpret_cast<float *>(smem + SH::M_OFF) + (n & 1) * RT * 4;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float v = warp_sum_butterfly(l[r]);
+        if (lane == 0) red[r * 4 + warp] = v;
+      }
+      ok = warpgroup_and(1, ok);
+      const bool whole = w.b == 0 && w.e == w.nb;
+      if (ok) {
+        const int slot = blockIdx.x * 2 + (w.b > 0 ? 0 : 1);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if (r >= rows) break;
+          const float4 v = *reinterpret_cast<const float4 *>(red + r * 4);
+          const float den = (v.x + v.y) + (v.z + v.w);
+          if (whole) {
+            int token, sub;
+            kv_row(a, row0 + r, token, sub);
+            if (tid < a.head_dim)
+              store_from_float(static_cast<T *>(a.out) + (w.q.c0 + static_cast<int64_t>(token)) * a.o_token +
+                                   static_cast<int64_t>(w.head * a.group + sub) * a.o_head + tid,
+                               den == 0.0f ? 0.0f : __fdividef(acc[r], den));
+          } else {
+            float *dst = a.ws + (static_cast<int64_t>(slot) * RT + r) * (D + 4);
+            dst[4 + tid] = acc[r];
+            if (tid == 0) dst[0] = m[r], dst[1] = den;
+          }
+        }
+      }
+      if (tid == 0 && min_blocks != 0) {
+        int4 *mt = a.meta + blockIdx.x;
+        if (pieces == 0) *mt = make_int4(-1, 0, 0, 0);
+        if (w.b > 0) mt->w = w.e == w.nb;
+        if (w.b == 0 && !whole) mt->x = w.s, mt->y = w.tile, mt->z = w.head;
+      }
+      ++pieces;
+      if (!ok) break;
+      w.next(c, bt, a);
+    }
+  } else if (warp == 4) {
+    // ================================================================ loads
+    const int box = min(c.page_size, SH::KEYS), boxes = SH::KEYS / box;  // rows of a box, boxes of a tile
+    const int in_page = (c.page_size >> 4) - 1;
+    uint32_t n = 0;
+    const auto entry = [&](int j) {  // lane i % 8: the table's entry for the tile's block i
+      return w.left > 0 ? kv_entry(c, bt, w.s, j * 8 + (lane & 7), w.q.len) : -1;
+    };
+    int32_t next_page = entry(w.b);
+    bool ok = true;
+    while (w.left > 0 && ok) {
+      for (int j = w.b; j < w.e; ++j, ++n) {
+        const int st = n % SH::STAGES;
+        const int32_t page = next_page;
+        const bool has = kv_page_ok(c, page, j * 8 + (lane & 7), w.q.len);
+        const uint32_t valid = __ballot_sync(0xffffffffu, has) & 0xFFu;
+        // ---- block scales: lanes 0-7 of K, 8-15 of V (on their way while the stage is waited for)
+        const int blk = (j * 8 + (lane & 7)) & in_page;
+        const float s = has && lane < 16 ? *c.scale(page, lane >> 3, w.head, blk) : 0.0f;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->empty[st], ((n / SH::STAGES) & 1) ^ 1));
+        if (!ok) break;
+        // ---- boxes: lane i brings box i of K and of V
+        const int first = lane * (box >> 4);  // the box's first block
+        const int32_t pg = __shfl_sync(0xffffffffu, page, first & 7);
+        if (lane < boxes && (valid >> first & 1)) {
+          const int32_t y = ((pg * 2) * c.kv_heads + w.head) * c.page_size + ((j * 8 + first) & in_page) * KV_BLOCK;
+          tma_load_2d(&map, &bar->full[st], smem + SH::K_OFF + st * SH::TILE + lane * box * 128, 0, y);
+          tma_load_2d(&map, &bar->full[st], smem + SH::V_OFF + st * SH::TILE + lane * box * 128, 0,
+                      y + c.kv_heads * c.page_size);
+        }
+        const bool more = j + 1 < w.e;
+        if (more) next_page = entry(j + 1);
+        const float top = redux_max(lane >= 8 && lane < 16 ? s : 0.0f);
+        KdFactors *fac = reinterpret_cast<KdFactors *>(smem + SH::F_OFF + st * 80);
+        if (lane < 8) fac->k[lane] = s * a.scale_log2;
+        if (lane >= 8 && lane < 16) fac->v[lane - 8] = top > 0.0f ? __fdiv_rn(s, top) * 127.0f : 0.0f;
+        if (lane == 16) fac->unit = __fdiv_rn(top, 127.0f), fac->blocks = valid;
+        int bytes = 0;
+        for (int i = 0; i < boxes; ++i) bytes += (valid >> (i * (box >> 4)) & 1) * box * 256;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&bar->full[st], bytes);
+      }
+      w.next(c, bt, a);
+      next_page = entry(w.b);
+    }
+  } else {
+    // ================================================================ MMA issue
+    if (lane == 0) {
+      const uint64_t q0 = make_sw128_desc(smem_u32(smem + SH::Q_OFF), 16, 1024);
+      const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
+      uint32_t n = 0, pieces = 0;
+      bool ok = true;
+      const auto scores = [&](uint32_t i) {
+        const int st = i % SH::STAGES;
+        if (!mbar_wait(&bar->full[st], (i / SH::STAGES) & 1)) return false;
+        tc_fence_after();
+        const uint64_t k0 = make_sw128_desc(smem_u32(smem + SH::K_OFF + st * SH::TILE), 16, 1024);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          umma_i8(tmem + (i & 1) * N, k0 + x * 2, q0 + x * 2, SH::IDESC, x > 0);
+        umma_commit(&bar->s_full[i & 1]);
+        return true;
+      };
+      while (n < total && ok) {
+        ok = mbar_wait(&bar->q_full, pieces & 1);
+        ++pieces;
+        if (!ok) break;
+        tc_fence_after();
+        const int tiles = bar->tiles;
+        ok = scores(n);
+        for (int i = 0; i < tiles && ok; ++i, ++n) {
+          if (i + 1 < tiles) ok = scores(n + 1);
+          ok = ok && mbar_wait(&bar->p_full[n & 1], (n >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const int st = n % SH::STAGES;
+          const uint64_t v0 = make_sw128_desc(smem_u32(smem + SH::V_OFF + st * SH::TILE), SH::TILE, 1024);
+          const uint64_t p0 = make_sw128_desc(smem_u32(smem + SH::P_OFF + (n & 1) * SH::ROWS), 16, 1024);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)  // 32 keys each
+            umma_i8(tmem + 2 * N + (n & 1) * N, v0 + x * (32 * 128 >> 4), p0 + x * 2, SH::IDESC_V, x > 0);
+          umma_commit(&bar->o_full[n & 1]);
+          umma_commit(&bar->empty[st]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, SH::TMEM);
+}
+
+}  // namespace rt

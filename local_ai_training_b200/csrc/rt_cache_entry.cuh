@@ -38,6 +38,20 @@ inline int kv_allow_smem(K *kernel, int bytes, std::mutex &mu, bool (&done)[64])
   return RT_OK;
 }
 
+// Row tiles of a batch, at most: a partly filled one per sequence with rows, and one per token while a
+// token's rows fit a tile.
+inline int64_t kv_most_tiles(const KvBatch &bt, int group, int tile) {
+  const int64_t some = std::min(bt.n_tokens, bt.n_seqs);
+  const int64_t tiles = (bt.n_tokens * group + some * (tile - 1)) / tile;
+  return group <= tile ? std::min(tiles, bt.n_tokens) : tiles;
+}
+// Few and short units take one CTA each and no join, whose launch would cost more than the few tokens that a
+// CTA then takes: at most `shortest`.  Returns their number, or 0 when the line is to be cut.
+inline int64_t kv_whole_units(const KvCache &c, const KvBatch &bt, const KvAttn &a, int tile, int ctas, int shortest) {
+  const int64_t units = kv_most_tiles(bt, a.group, tile) * c.kv_heads;
+  return units <= ctas && bt.pages_per_seq * c.page_size <= shortest ? units : 0;
+}
+
 template <typename T, int D, int NT>
 int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
   using SH = KaShape<T, D, NT>;
@@ -45,21 +59,35 @@ int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int s
   static bool done[64] = {false};
   auto *kernel = kv_attention_kernel<T, D, NT>;
   if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
-  // Few and short units: one CTA each and no join, whose launch costs more than the 8 blocks, at most, that
-  // each warp then takes.  Row tiles of a batch, at most: a partly filled one per sequence with rows,
-  // and one per token while a token's rows fit a tile.
-  const int64_t rows = bt.n_tokens * a.group, some = std::min(bt.n_tokens, bt.n_seqs);
-  int64_t units = (rows + some * (SH::RT - 1)) / SH::RT;
-  if (a.group <= SH::RT) units = std::min(units, bt.n_tokens);
-  units *= c.kv_heads;
   const int ctas = sms * SH::MIN_CTAS;
-  if (units > 0 && units <= ctas && bt.pages_per_seq * c.page_size <= 64 * KV_BLOCK) {
+  if (const int64_t units = kv_whole_units(c, bt, a, SH::RT, ctas, 1024)) {
     launch_k(kernel, static_cast<unsigned>(units), KA_WARPS * 32, SH::SMEM, s, c, bt, a, 0);
     return check_launch("kv_attention");
   }
   launch_k(kernel, ctas, KA_WARPS * 32, SH::SMEM, s, c, bt, a, KA_WARPS);
-  launch_k(kv_attention_join_kernel<T, D, SH::RT>, dim3(ctas, SH::RT / 8), 256, 0, s, c, bt,
-           a, ctas);
+  launch_k(kv_attention_join_kernel<T, D, SH::RT>, dim3(ctas, SH::RT / 8), 256, 0, s, c, bt, a, ctas);
+  return check_launch("kv_attention");
+}
+template <typename T, int RT>
+int kv_decode_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+  using SH = KdShape<T, RT>;
+  static std::mutex mu;
+  static bool done[64] = {false};
+  auto *kernel = kv_decode_kernel<T, RT>;
+  if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
+  const int64_t rows = c.n_pages * 2 * c.kv_heads * c.page_size;
+  if (rows > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "kv_attention: cache too large");
+  CUtensorMap map;
+  if (int rc = make_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.codes, 128, rows, 128, 128,
+                        std::min(c.page_size, SH::KEYS)))
+    return rc;
+  const int ctas = sms * SH::CTAS;
+  if (const int64_t units = kv_whole_units(c, bt, a, RT, ctas, 512)) {
+    launch_k(kernel, static_cast<unsigned>(units), 192, SH::SMEM, s, map, c, bt, a, 0);
+    return check_launch("kv_attention");
+  }
+  launch_k(kernel, ctas, 192, SH::SMEM, s, map, c, bt, a, 2);
+  launch_k(kv_attention_join_kernel<T, 128, RT>, dim3(ctas, (RT + 7) / 8), 256, 0, s, c, bt, a, ctas);
   return check_launch("kv_attention");
 }
 template <int D>
@@ -76,15 +104,16 @@ int kv_prefill_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms
 }
 template <typename T>
 int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
-  // 16-row tiles once the sequences average more than 8 rows per kv head
-  const bool wide = bt.n_tokens * a.group > 8 * bt.n_seqs;
+  // row tiles by the rows that the sequences average per kv head
+  const int64_t rows = bt.n_tokens * a.group;
+  const bool wide = rows > 8 * bt.n_seqs;
   switch (c.dim) {
     case 32:
       return wide ? kv_attention_run<T, 32, 2>(c, bt, a, sms, s) : kv_attention_run<T, 32, 1>(c, bt, a, sms, s);
     case 64:
       return wide ? kv_attention_run<T, 64, 2>(c, bt, a, sms, s) : kv_attention_run<T, 64, 1>(c, bt, a, sms, s);
     case 128:
-      return wide ? kv_attention_run<T, 128, 2>(c, bt, a, sms, s) : kv_attention_run<T, 128, 1>(c, bt, a, sms, s);
+      return rows > 4 * bt.n_seqs ? kv_decode_run<T, 16>(c, bt, a, sms, s) : kv_decode_run<T, 4>(c, bt, a, sms, s);
     default:
       return kv_attention_run<T, 256, 1>(c, bt, a, sms, s);
   }

@@ -17,7 +17,7 @@
 // maximum moves, and O is rescaled, only when a score exceeds it by 2^8.
 #pragma once
 
-#include "rt_cache_attn.cuh"
+#include "rt_cache_decode.cuh"
 
 namespace rt {
 
@@ -39,18 +39,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// 16 columns, loaded and waited for.
-__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
 // 16 bytes global -> shared, zeros when `in` is false.
 __device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void *gmem, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0)
@@ -63,19 +51,6 @@ __device__ __forceinline__ void set_registers_up() {
 template <int N>
 __device__ __forceinline__ void set_registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-// Barrier of 128 threads (one row tile's softmax warps) that also ands a flag over them.
-__device__ __forceinline__ bool warpgroup_and(int id, bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(static_cast<uint32_t>(v))
-      : "memory");
-  return r != 0;
 }
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -425,7 +400,7 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
       const float l = l2.x + l2.y;
       if (ok) {
         const int slot = blockIdx.x * 2 + (w.b > 0 ? 0 : 1);
-        const float scale = !whole ? 1.0f : l > 0.0f ? __fdividef(1.0f, l) : 0.0f;
+        const float scale = !whole ? 1.0f : l == 0.0f ? 0.0f : __fdividef(1.0f, l);
         uint8_t *stage = smem + SH::Q_OFF + x * SH::TILE;
         float *ws = a.ws + (static_cast<int64_t>(slot) * SH::RT + x * SH::ROWS) * (D + 4);
         if (!whole && r < rows) *reinterpret_cast<float2 *>(ws + static_cast<int64_t>(r) * (D + 4)) = make_float2(m, l);

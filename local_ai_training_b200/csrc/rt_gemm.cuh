@@ -20,6 +20,7 @@
 #include <mutex>
 
 #include "rt_common.cuh"
+#include "rt_tensormap.cuh"
 
 namespace rt {
 
@@ -805,42 +806,6 @@ __global__ void simt_matmul_bf16_kernel(const uint16_t *a, int64_t lda, const ui
 // -------------------------------------------------------------------------------------------
 // Host side: tensor maps (driver entry point fetched once), launch helpers.
 // -------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                   const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                   const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
-}
-
-// 2-D map over a row-major matrix: `inner` contiguous elements per row, `outer` rows,
-// `row_bytes` between rows; box = box_inner × box_outer with 128-byte swizzle, zero OOB fill.
-static int make_map(CUtensorMap *map, CUtensorMapDataType dt, const void *base, uint64_t inner,
-                    uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer) {
-  EncodeTiledFn enc = encode_fn();
-  if (enc == nullptr) return fail(RT_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_bytes};
-  const cuuint32_t box[2] = {box_inner, box_outer};
-  const cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, dt, 2, const_cast<void *>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(RT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
-  return RT_OK;
-}
-
 // Operand description for the UMMA path.  A is (M,K), B is (N,K) in GEMM terms.
 struct Operand {
   const void *ptr;
