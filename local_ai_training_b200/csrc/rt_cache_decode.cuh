@@ -12,9 +12,9 @@
 //   O^T [128 dims x N] = V^T (the tile as it lies, M-major) · P^T (N rows of digits over the keys)
 // Products and sums are exact (|sum| < 2^21); a thread is a key in S^T and a dim in O^T, so it holds all
 // digits of its rows and joins them in fp32.  O is summed in registers, rescaled as m moves.
-//   warps 0-3  scores -> weights -> digits; sums of O, a tile behind, while the tensor core works
-//   warp 4     TMA: page entries, tiles of 128 keys of K and V, block scales
-//   warp 5     one thread issues the products, the next tile's scores before this one's outputs
+//   warps 0-3 (0-7 for 16 rows: eight rows each)  scores -> weights -> digits; sums of O, a tile behind, while the tensor core works
+//   the next warp  TMA: page entries, tiles of 128 keys of K and V, block scales
+//   the last warp  one thread issues the products, the next tile's scores before this one's outputs
 #pragma once
 
 #include "rt_cache_attn.cuh"
@@ -71,6 +71,9 @@ struct KdShape {
   static constexpr int QS_OFF = M_OFF + 2 * RT * 16;      // qs of the rows
   static constexpr int BAR_OFF = QS_OFF + RT * 4;
   static constexpr int SMEM = BAR_OFF + 256 + 1024;
+  static constexpr int GROUPS = RT == 16 ? 2 : 1;         // softmax warpgroups, which share the rows
+  static constexpr int RW = RT / GROUPS;                  // rows of one
+  static constexpr int THREADS = 128 * GROUPS + 64;
   static constexpr int TMEM = N == 16 ? 64 : 256;         // two S and two O tiles of N columns
   static constexpr int CTAS = 2;                          // per SM
   static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((128 >> 4) << 24);
@@ -102,20 +105,44 @@ __device__ __forceinline__ uint32_t digits_of(float x) {
   }
   return w;
 }
-template <int ND, int RT>
-__device__ __forceinline__ float joined(const uint32_t *s, int r) {
-  float v = small_int(s[(ND - 1) * RT + r]);
+// The digits' columns of RW rows, loaded together and waited for: column i · RT + r to s[i][r].
+template <int ND, int RT, int RW>
+__device__ __forceinline__ void load_digits(uint32_t taddr, uint32_t (&s)[ND][RW]) {
+  if constexpr (RT == 4) {  // sixteen columns hold them all
+    uint32_t a[16];
+    tmem_ld_32x32b_x16(taddr, a);
 #pragma unroll
-  for (int i = ND - 2; i >= 0; --i) v = fmaf(v, 0.0078125f, small_int(s[i * RT + r]));
+    for (int i = 0; i < ND * 4; ++i) s[i / 4][i % 4] = a[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    uint32_t(&r)[RW] = s[i];
+    if constexpr (RW == 8)
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                   : "r"(taddr + i * RT));
+  }
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < ND; ++i)  // no use of the registers before the wait
+#pragma unroll
+    for (int r = 0; r < RW; ++r) asm volatile("" : "+r"(s[i][r])::"memory");
+}
+template <int ND, int RW>
+__device__ __forceinline__ float joined(const uint32_t (&s)[ND][RW], int r) {
+  float v = small_int(s[ND - 1][r]);
+#pragma unroll
+  for (int i = ND - 2; i >= 0; --i) v = fmaf(v, 0.0078125f, small_int(s[i][r]));
   return v;
 }
 
 template <typename T, int RT>
-__global__ void __launch_bounds__(192, 2)
+__global__ void __launch_bounds__(KdShape<T, RT>::THREADS, 2)
     kv_decode_kernel(const __grid_constant__ CUtensorMap map, KvCache c, KvBatch bt, KvAttn a, int min_blocks) {
   using SH = KdShape<T, RT>;
   using Walk = KvWalk<RT, SH::KEYS>;
-  constexpr int ND = SH::ND, N = SH::N, D = SH::D;
+  constexpr int ND = SH::ND, N = SH::N, D = SH::D, RW = SH::RW, W4 = 4 * SH::GROUPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   KdBars *bar = reinterpret_cast<KdBars *>(smem + SH::BAR_OFF);
@@ -123,40 +150,43 @@ __global__ void __launch_bounds__(192, 2)
   if (tid == 0) {
     for (int i = 0; i < SH::STAGES; ++i) mbar_init(&bar->full[i], 1), mbar_init(&bar->empty[i], 1);
     for (int i = 0; i < 2; ++i)
-      mbar_init(&bar->s_full[i], 1), mbar_init(&bar->p_full[i], 128), mbar_init(&bar->o_full[i], 1);
-    mbar_init(&bar->q_full, 128);
+      mbar_init(&bar->s_full[i], 1), mbar_init(&bar->p_full[i], 128 * SH::GROUPS), mbar_init(&bar->o_full[i], 1);
+    mbar_init(&bar->q_full, 128 * SH::GROUPS);
     fence_barrier_init();
     tma_prefetch_desc(&map);
   }
-  if (warp == 5) {
+  if (warp == W4 + 1) {
     tmem_alloc(&bar->tmem, SH::TMEM);
     tmem_relinquish();
   }
   pdl_wait();
   kv_zero_rest<T>(bt, a);
   Walk w;
-  const bool busy = kv_walk_start<192>(w, c, bt, a, min_blocks);
+  const bool busy = kv_walk_start<SH::THREADS>(w, c, bt, a, min_blocks);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   pdl_trigger();  // the next kernel comes up only now that this one has its tensor memory
   if (!busy) {
     if (tid == 0 && min_blocks != 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    if (warp == 5) tmem_dealloc(bar->tmem, SH::TMEM);
+    if (warp == W4 + 1) tmem_dealloc(bar->tmem, SH::TMEM);
     return;
   }
   const uint32_t tmem = bar->tmem;
 
-  if (warp < 4) {
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp) << 21);
+  if (warp < W4) {
+    const int key_row = tid & 127;  // this thread's key of a tile, and its dim of the outputs
+    const int first_row = (warp >> 2) * RW, wq = warp & 3;  // the warpgroup's rows of the unit
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(wq) << 21) + first_row;
     float *qs = reinterpret_cast<float *>(smem + SH::QS_OFF);
     uint32_t n = 0, pieces = 0;  // tiles of the CTA
     bool ok = true;
     while (w.left > 0) {
-      const int row0 = w.tile * RT, rows = min(RT, w.q.n * a.group - row0);
+      const int row0 = w.tile * RT + first_row;  // of the sequence
+      const int rows = max(min(RW, w.q.n * a.group - row0), 0);
       // ---- q's digits: a warp per row, four dims a lane
 #pragma unroll 1
-      for (int r = warp; r < RT; r += 4) {
+      for (int r = wq; r < RW; r += 4) {
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (r < rows) {
           int token, sub;
@@ -185,13 +215,13 @@ __global__ void __launch_bounds__(192, 2)
         amax = redux_max(amax);
         // (a row below 2^-100 scores nothing; a row with an infinity or a NaN makes its scores NaN)
         const float inv = amax > 7.8e-31f ? __fdiv_rn(127.0f, amax) : 0.0f;
-        if (lane == 0) qs[r] = odd ? __int_as_float(0x7FC00000) : __fdiv_rn(amax, 127.0f);
+        if (lane == 0) qs[first_row + r] = odd ? __int_as_float(0x7FC00000) : __fdiv_rn(amax, 127.0f);
         uint32_t w4[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w4[i] = digits_of<ND>(fminf(fmaxf(x[i] * inv, -127.0f), 127.0f));
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
-          const int row = i * RT + r;
+          const int row = i * RT + first_row + r;
           const uint32_t word = (w4[0] >> 8 * i & 0xFFu) | (w4[1] >> 8 * i & 0xFFu) << 8 |
                                 (w4[2] >> 8 * i & 0xFFu) << 16 | (w4[3] >> 8 * i & 0xFFu) << 24;
           *reinterpret_cast<uint32_t *>(smem + SH::Q_OFF + row * 128 + ((lane * 4) ^ ((row & 7) << 4))) = word;
@@ -201,21 +231,19 @@ __global__ void __launch_bounds__(192, 2)
       fence_proxy_async_smem();
       tc_fence_before();
       mbar_arrive(&bar->q_full);
-      ok = warpgroup_and(1, ok);  // qs of all rows
+      ok = warpgroup_and(1 + (warp >> 2), ok);  // qs of all rows
 
-      float m[RT], l[RT], acc[RT], f[RT], unit = 0.0f;
+      float m[RW], l[RW], acc[RW], unit = 0.0f;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) m[r] = -1e30f, l[r] = acc[r] = f[r] = 0.0f;
-      // adds the outputs of tile i, whose weights were under the maximum before f's move
-      const auto add_outputs = [&](uint32_t i) {
+      for (int r = 0; r < RW; ++r) m[r] = -1e30f, l[r] = acc[r] = 0.0f;
+      // adds the outputs of tile i, then follows the maxima's move by g
+      const auto add_outputs = [&](uint32_t i, const float (&g)[RW]) {
         ok = mbar_wait(&bar->o_full[i & 1], (i >> 1) & 1) && ok;
         tc_fence_after();
-        uint32_t o[N];
+        uint32_t o[ND][RW];
+        load_digits<ND, RT, RW>(t_lane + 2 * N + (i & 1) * N, o);
 #pragma unroll
-        for (int x = 0; x < N / 16; ++x)
-          tmem_ld_32x32b_x16(t_lane + 2 * N + (i & 1) * N + x * 16, *reinterpret_cast<uint32_t(*)[16]>(o + x * 16));
-#pragma unroll
-        for (int r = 0; r < RT; ++r) acc[r] = fmaf(acc[r], f[r], joined<ND, RT>(o, r) * unit);
+        for (int r = 0; r < RW; ++r) acc[r] = fmaf(joined(o, r), unit, acc[r]) * g[r];
       };
 #pragma unroll 1
       for (int j = w.b; j < w.e && ok; ++j, ++n) {
@@ -223,35 +251,33 @@ __global__ void __launch_bounds__(192, 2)
         ok = mbar_wait(&bar->full[st], (n / SH::STAGES) & 1) && mbar_wait(&bar->s_full[n & 1], (n >> 1) & 1);
         tc_fence_after();
         const KdFactors *fac = reinterpret_cast<const KdFactors *>(smem + SH::F_OFF + st * 80);
-        const float fk = fac->k[tid >> 4], fv = fac->v[tid >> 4], unit_now = fac->unit;
-        const bool has = fac->blocks >> (tid >> 4) & 1;
-        float t[RT];
+        const float fk = fac->k[key_row >> 4], fv = fac->v[key_row >> 4], unit_now = fac->unit;
+        const bool has = fac->blocks >> (key_row >> 4) & 1;
+        float t[RW];
         {
-          uint32_t s[N];
+          uint32_t s[ND][RW];
+          load_digits<ND, RT, RW>(t_lane + (n & 1) * N, s);
 #pragma unroll
-          for (int x = 0; x < N / 16; ++x)
-            tmem_ld_32x32b_x16(t_lane + (n & 1) * N + x * 16, *reinterpret_cast<uint32_t(*)[16]>(s + x * 16));
-#pragma unroll
-          for (int r = 0; r < RT; ++r) t[r] = joined<ND, RT>(s, r) * (fk * qs[r]);
+          for (int r = 0; r < RW; ++r) t[r] = joined(s, r) * (fk * qs[first_row + r]);
         }
-        const int key = j * SH::KEYS + tid;
+        const int key = j * SH::KEYS + key_row;
         if ((j + 1) * SH::KEYS > w.seen(a, row0 + 1) || fac->blocks != 0xFFu) {  // a key some row does not see
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            if (!has || key >= w.seen(a, row0 + min(r, rows - 1) + 1)) t[r] = -INFINITY;
+          for (int r = 0; r < RW; ++r)
+            if (!has || key >= w.seen(a, row0 + min(r, max(rows - 1, 0)) + 1)) t[r] = -INFINITY;
         }
-        float *mx = reinterpret_cast<float *>(smem + SH::M_OFF) + (n & 1) * RT * 4;
+        float *mx = reinterpret_cast<float *>(smem + SH::M_OFF) + ((n & 1) * RT + first_row) * 4;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int r = 0; r < RW; ++r) {
           const float v = redux_max(t[r]);
-          if (lane == r) mx[r * 4 + warp] = v;
+          if (lane == r) mx[r * 4 + wq] = v;
         }
-        ok = warpgroup_and(1, ok);
+        ok = warpgroup_and(1 + (warp >> 2), ok);
         if (!ok) break;
         uint8_t *pt = smem + SH::P_OFF + (n & 1) * SH::ROWS;
-        float g[RT];  // how far the maxima move
+        float g[RW];  // how far the maxima move
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int r = 0; r < RW; ++r) {
           const float4 v = *reinterpret_cast<const float4 *>(mx + r * 4);
           const float mn = fmaxf(m[r], fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
           g[r] = ex2(m[r] - mn);
@@ -261,46 +287,49 @@ __global__ void __launch_bounds__(192, 2)
           const uint32_t dg = digits_of<ND>(p * fv);
 #pragma unroll
           for (int i = 0; i < ND; ++i) {
-            const int row = i * RT + r;
-            pt[row * 128 + (tid ^ ((row & 7) << 4))] = static_cast<uint8_t>(dg >> (8 * i));
+            const int row = i * RT + first_row + r;
+            pt[row * 128 + (key_row ^ ((row & 7) << 4))] = static_cast<uint8_t>(dg >> (8 * i));
           }
         }
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(&bar->p_full[n & 1]);
-        if (j > w.b) add_outputs(n - 1);
+        if (j > w.b) add_outputs(n - 1, g);
         unit = unit_now;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) f[r] = g[r];
       }
       // ---- the piece's rows: thread = dim
-      if (ok) add_outputs(n - 1);
-      float *red = reinterpret_cast<float *>(smem + SH::M_OFF) + (n & 1) * RT * 4;
+      if (ok) {
+        float one[RW];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const float v = warp_sum_butterfly(l[r]);
-        if (lane == 0) red[r * 4 + warp] = v;
+        for (int r = 0; r < RW; ++r) one[r] = 1.0f;
+        add_outputs(n - 1, one);
       }
-      ok = warpgroup_and(1, ok);
+      float *red = reinterpret_cast<float *>(smem + SH::M_OFF) + ((n & 1) * RT + first_row) * 4;
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        const float v = warp_sum_butterfly(l[r]);
+        if (lane == 0) red[r * 4 + wq] = v;
+      }
+      ok = warpgroup_and(1 + (warp >> 2), ok);
       const bool whole = w.b == 0 && w.e == w.nb;
       if (ok) {
         const int slot = blockIdx.x * 2 + (w.b > 0 ? 0 : 1);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int r = 0; r < RW; ++r) {
           if (r >= rows) break;
           const float4 v = *reinterpret_cast<const float4 *>(red + r * 4);
           const float den = (v.x + v.y) + (v.z + v.w);
           if (whole) {
             int token, sub;
             kv_row(a, row0 + r, token, sub);
-            if (tid < a.head_dim)
+            if (key_row < a.head_dim)
               store_from_float(static_cast<T *>(a.out) + (w.q.c0 + static_cast<int64_t>(token)) * a.o_token +
-                                   static_cast<int64_t>(w.head * a.group + sub) * a.o_head + tid,
+                                   static_cast<int64_t>(w.head * a.group + sub) * a.o_head + key_row,
                                den == 0.0f ? 0.0f : __fdividef(acc[r], den));
           } else {
-            float *dst = a.ws + (static_cast<int64_t>(slot) * RT + r) * (D + 4);
-            dst[4 + tid] = acc[r];
-            if (tid == 0) dst[0] = m[r], dst[1] = den;
+            float *dst = a.ws + (static_cast<int64_t>(slot) * RT + first_row + r) * (D + 4);
+            dst[4 + key_row] = acc[r];
+            if (key_row == 0) dst[0] = m[r], dst[1] = den;
           }
         }
       }
@@ -314,7 +343,7 @@ __global__ void __launch_bounds__(192, 2)
       if (!ok) break;
       w.next(c, bt, a);
     }
-  } else if (warp == 4) {
+  } else if (warp == W4) {
     // ================================================================ loads
     const int box = min(c.page_size, SH::KEYS), boxes = SH::KEYS / box;  // rows of a box, boxes of a tile
     const int in_page = (c.page_size >> 4) - 1;
@@ -405,7 +434,7 @@ __global__ void __launch_bounds__(192, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, SH::TMEM);
+  if (warp == W4 + 1) tmem_dealloc(tmem, SH::TMEM);
 }
 
 }  // namespace rt

@@ -14,9 +14,12 @@ inline int kv_sm_count() {
 constexpr int KA_GRID = 2;       // CTAs per SM of the few-row kernel, at most
 constexpr int KP_MIN_ROWS = 64;  // rows per kv head from which a sequence takes the tcgen05 kernel
 
-// Whether any sequence of the batch can take the tcgen05 kernel.
-inline bool kv_prefill_fits(int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t dim) {
-  return (dim == 64 || dim == 128) && n_tokens * (q_heads / kv_heads) >= KP_MIN_ROWS;
+// Whether a sequence of the batch may take the tcgen05 kernel: one that has the batch to itself, or all
+// tokens but one for each of the others.  (A batch of as many tokens as sequences is a decode step; one
+// that is not so after all is computed by the few-row kernels.)
+inline bool kv_prefill_fits(int64_t n_seqs, int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t dim) {
+  const int64_t most = n_tokens - std::max<int64_t>(n_seqs - 1, 0);
+  return (dim == 64 || dim == 128) && most * (q_heads / kv_heads) >= KP_MIN_ROWS;
 }
 inline int64_t kv_few_bytes(int64_t sms, int64_t dim) {
   return sms * KA_GRID * (16 + 2 * 16 * (dim + 4) * 4);
@@ -83,10 +86,10 @@ int kv_decode_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms,
     return rc;
   const int ctas = sms * SH::CTAS;
   if (const int64_t units = kv_whole_units(c, bt, a, RT, ctas, 512)) {
-    launch_k(kernel, static_cast<unsigned>(units), 192, SH::SMEM, s, map, c, bt, a, 0);
+    launch_k(kernel, static_cast<unsigned>(units), SH::THREADS, SH::SMEM, s, map, c, bt, a, 0);
     return check_launch("kv_attention");
   }
-  launch_k(kernel, ctas, 192, SH::SMEM, s, map, c, bt, a, 2);
+  launch_k(kernel, ctas, SH::THREADS, SH::SMEM, s, map, c, bt, a, 2);
   launch_k(kv_attention_join_kernel<T, 128, RT>, dim3(ctas, (RT + 7) / 8), 256, 0, s, c, bt, a, ctas);
   return check_launch("kv_attention");
 }
@@ -125,11 +128,10 @@ using namespace rt;
 
 extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
                                                    int64_t kv_heads, int64_t padded_dim) {
-  (void)n_seqs;
   if (kv_heads <= 0 || n_tokens <= 0) return 0;
   const int64_t sms = kv_sm_count();
   return kv_few_bytes(sms, padded_dim) +
-         (kv_prefill_fits(n_tokens, q_heads, kv_heads, padded_dim) ? kv_prefill_bytes(sms, padded_dim) : 0);
+         (kv_prefill_fits(n_seqs, n_tokens, q_heads, kv_heads, padded_dim) ? kv_prefill_bytes(sms, padded_dim) : 0);
 }
 
 extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
@@ -182,7 +184,7 @@ extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
   a.rows_lo = 0, a.rows_hi = INT32_MAX;
   // Rows are known on the device only: a batch that may hold sequences of both kinds launches both
   // kernels, and each takes its own sequences.  One sequence is a prompt piece when it is long enough.
-  const bool prefill = dtype == RT_BF16 && kv_prefill_fits(n_tokens, q_heads, kv_heads, padded_dim);
+  const bool prefill = dtype == RT_BF16 && kv_prefill_fits(n_seqs, n_tokens, q_heads, kv_heads, padded_dim);
   cudaStream_t s = as_stream(stream);
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   if (prefill) {
