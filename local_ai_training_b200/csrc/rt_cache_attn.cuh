@@ -120,7 +120,8 @@ struct KvWalk {
 
   // keys that the first `rows` rows of the sequence see
   __device__ __forceinline__ int seen(const KvAttn &a, int rows) const {
-    return min(max(q.start + (rows - 1) / a.group + 1, 0), q.len);
+    const int token = a.group_shift >= 0 ? (rows - 1) >> a.group_shift : (rows - 1) / a.group;
+    return min(max(q.start + token + 1, 0), q.len);
   }
   __device__ __forceinline__ void set_tile(const KvAttn &a) {
     nb = max((seen(a, min((tile + 1) * RT, q.n * a.group)) + KEYS - 1) / KEYS, 1);
@@ -130,12 +131,12 @@ struct KvWalk {
     const int rows = q.n * a.group;
     tiles = rows >= a.rows_lo && rows < a.rows_hi ? (rows + RT - 1) / RT : 0;
   }
-  // Blocks of sequence s over all its row tiles (one kv head).
-  __device__ __forceinline__ int64_t seq_blocks(const KvCache &c, const KvBatch &bt, const KvAttn &a,
-                                                bool units = false) {
+  // Blocks of sequence s over all its row tiles (one kv head), or its units.
+  __device__ __forceinline__ int seq_blocks(const KvCache &c, const KvBatch &bt, const KvAttn &a, bool units) {
     set_seq(c, bt, a);
-    if (units) return tiles;  // units instead of blocks
-    int64_t sum = 0;
+    if (units) return tiles;
+    int sum = 0;
+#pragma unroll 1
     for (tile = 0; tile < tiles; ++tile) {
       set_tile(a);
       sum += nb;
@@ -172,52 +173,59 @@ template <int THREADS, int RT, int KEYS>
 __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache &c, const KvBatch &bt,
                                               const KvAttn &a, int min_blocks) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ int64_t sm_sum[WARPS];
-  __shared__ int sm_start[5];
+  __shared__ int sm_sum[WARPS], sm_start[5];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool units = min_blocks == 0;
-  const int per = static_cast<int>((bt.n_seqs + THREADS - 1) / THREADS);
-  const int s0 = min(tid * per, static_cast<int>(bt.n_seqs));
-  const int s1 = min(s0 + per, static_cast<int>(bt.n_seqs));
-  int64_t mine = 0;
+  // a thread's sequences (one each, up to THREADS of them); the line's length fits 31 bits (host check)
+  const int seqs = static_cast<int>(bt.n_seqs), per = seqs <= THREADS ? 1 : (seqs + THREADS - 1) / THREADS;
+  const int s0 = min(tid * per, seqs), s1 = min(s0 + per, seqs);
+  int mine = 0;
+#pragma unroll 1
   for (w.s = s0; w.s < s1; ++w.s) mine += w.seq_blocks(c, bt, a, units);
   mine *= c.kv_heads;
-  int64_t scan = mine;
+  int scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, scan, o);
+    const int v = __shfl_up_sync(0xffffffffu, scan, o);
     if (lane >= o) scan += v;
   }
   if (lane == 31) sm_sum[warp] = scan;
   if (tid == 0) sm_start[0] = -1;
   __syncthreads();
-  int64_t before = scan - mine, total = 0;
+  int before = scan - mine, total = 0;
 #pragma unroll
   for (int i = 0; i < WARPS; ++i) {
     if (i < warp) before += sm_sum[i];
     total += sm_sum[i];
   }
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), units ? total : (total + min_blocks - 1) / min_blocks);
-  const int64_t p0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
-  const int64_t p1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
-  if (p0 < p1 && before <= p0 && p0 < before + mine) {  // one thread's sequences hold p0
-    int64_t at = before;
-    for (w.s = s0; w.s < s1 - 1; ++w.s) {
-      const int64_t n = w.seq_blocks(c, bt, a, units) * c.kv_heads;
-      if (p0 < at + n) break;
-      at += n;
+  const int cta = blockIdx.x;
+  const int ctas = min(static_cast<int>(gridDim.x), units ? total : (total + min_blocks - 1) / min_blocks);
+  if (cta < ctas) {
+    // shares [total · cta / ctas, total · (cta + 1) / ctas)
+    const int q = total / ctas, rest = total - q * ctas;
+    const int p0 = q * cta + rest * cta / ctas, p1 = q * (cta + 1) + rest * (cta + 1) / ctas;
+    if (p0 < p1 && before <= p0 && p0 < before + mine) {  // one thread's sequences hold p0
+      int at = before;
+      w.s = s0;
+#pragma unroll 1
+      while (w.s < s1 - 1) {
+        const int n = w.seq_blocks(c, bt, a, units) * c.kv_heads;
+        if (p0 < at + n) break;
+        at += n;
+        ++w.s;
+      }
+      w.set_seq(c, bt, a);
+      int per_head;
+#pragma unroll 1
+      for (w.tile = 0;; ++w.tile) {
+        w.set_tile(a);
+        per_head = units ? 1 : w.nb;
+        if (p0 < at + per_head * c.kv_heads || w.tile >= w.tiles - 1) break;
+        at += per_head * c.kv_heads;
+      }
+      sm_start[0] = w.s, sm_start[1] = w.tile, sm_start[2] = (p0 - at) / per_head;
+      sm_start[3] = p0 - at - sm_start[2] * per_head, sm_start[4] = units ? w.nb : p1 - p0;
     }
-    w.set_seq(c, bt, a);
-    for (w.tile = 0;; ++w.tile) {
-      w.set_tile(a);
-      const int64_t n = static_cast<int64_t>(units ? 1 : w.nb) * c.kv_heads;
-      if (p0 < at + n || w.tile >= w.tiles - 1) break;
-      at += n;
-    }
-    const int per_head = units ? 1 : w.nb;
-    sm_start[0] = w.s, sm_start[1] = w.tile;
-    sm_start[2] = static_cast<int>((p0 - at) / per_head), sm_start[3] = static_cast<int>((p0 - at) % per_head);
-    sm_start[4] = units ? w.nb : static_cast<int>(p1 - p0);
   }
   __syncthreads();
   if (sm_start[0] < 0) return false;
@@ -576,8 +584,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
 }
 
 // Joins the partial rows of every unit that a CTA began and did not end: its own, then those of the
-// following CTAs up to the one that ended the unit, in that order.  One warp per row, eight rows per
-// CTA (grid.y covers a unit's rows); lanes over the partials for the factors, then over the width.
+// following CTAs up to the one that ended the unit, in that order.  A warp takes a row at a time (grid.y
+// CTAs share a unit's rows); lanes over the partials for the factors, then over the width.
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBatch bt, KvAttn a, int ctas) {
   constexpr int W = D >= 128 ? 4 : D / 32, CH = D / (32 * W);  // floats of a lane's access, accesses
@@ -585,10 +593,9 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBat
   pdl_trigger();
   const int4 mt = a.meta[blockIdx.x];
   if (mt.x < 0) return;
-  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
   const KvSeq q = kv_seq(bt, c.page_size, mt.x);
-  const int row = mt.y * RT + r;
-  if (r >= RT || row >= q.n * a.group) return;
+  const int rows = min(RT, q.n * a.group - mt.y * RT);
   int last = blockIdx.x + 1;  // the CTA that ended the unit
   for (;; last += 32) {
     const int x = last + lane;
@@ -598,50 +605,54 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBat
       break;
     }
   }
-  const auto slot = [&](int cta) {
-    return a.ws + (static_cast<int64_t>(cta * 2 + (cta == static_cast<int>(blockIdx.x))) * RT + r) * (D + 4);
-  };
   const int first = blockIdx.x;
-  float top = -1e30f;
-  for (int x = first + lane; x <= last; x += 32) top = fmaxf(top, slot(x)[0]);
-  top = warp_max(top);
-  float den = 0.0f, acc[CH * W];
+#pragma unroll 1
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    const int row = mt.y * RT + r;
+    const auto slot = [&](int cta) {
+      return a.ws + (static_cast<int64_t>(cta * 2 + (cta == first)) * RT + r) * (D + 4);
+    };
+    float top = -1e30f;
+    for (int x = first + lane; x <= last; x += 32) top = fmaxf(top, slot(x)[0]);
+    top = warp_max(top);
+    float den = 0.0f, acc[CH * W];
 #pragma unroll
-  for (int i = 0; i < CH * W; ++i) acc[i] = 0.0f;
-  for (int x0 = first; x0 <= last; x0 += 32) {
-    float f = 0.0f;
-    if (x0 + lane <= last) {
-      const float2 ml = *reinterpret_cast<const float2 *>(slot(x0 + lane));
-      f = ex2(ml.x - top);
-      den += f * ml.y;
-    }
-    const int n = min(32, last + 1 - x0);
+    for (int i = 0; i < CH * W; ++i) acc[i] = 0.0f;
+    for (int x0 = first; x0 <= last; x0 += 32) {
+      float f = 0.0f;
+      if (x0 + lane <= last) {
+        const float2 ml = *reinterpret_cast<const float2 *>(slot(x0 + lane));
+        f = ex2(ml.x - top);
+        den += f * ml.y;
+      }
+      const int n = min(32, last + 1 - x0);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float g = __shfl_sync(0xffffffffu, f, i);
-      const float *p = slot(x0 + i) + 4 + lane * W;
+      for (int i = 0; i < n; ++i) {
+        const float g = __shfl_sync(0xffffffffu, f, i);
+        const float *p = slot(x0 + i) + 4 + lane * W;
 #pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        float v[W];
-        if constexpr (W == 4)
-          *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p + k * 128);
-        else if constexpr (W == 2)
-          *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
-        else
-          v[0] = *p;
+        for (int k = 0; k < CH; ++k) {
+          float v[W];
+          if constexpr (W == 4)
+            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p + k * 128);
+          else if constexpr (W == 2)
+            *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
+          else
+            v[0] = *p;
 #pragma unroll
-        for (int j = 0; j < W; ++j) acc[k * W + j] += g * v[j];
+          for (int j = 0; j < W; ++j) acc[k * W + j] += g * v[j];
+        }
       }
     }
-  }
-  den = warp_sum_butterfly(den);
-  const float inv = den == 0.0f ? 0.0f : __fdividef(1.0f, den);
-  T *o = static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(row / a.group)) * a.o_token +
-         static_cast<int64_t>(mt.z * a.group + row % a.group) * a.o_head;
+    den = warp_sum_butterfly(den);
+    const float inv = den == 0.0f ? 0.0f : __fdividef(1.0f, den);
+    T *o = static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(row / a.group)) * a.o_token +
+           static_cast<int64_t>(mt.z * a.group + row % a.group) * a.o_head;
 #pragma unroll
-  for (int i = 0; i < CH * W; ++i) {
-    const int d = (i / W) * 128 + lane * W + i % W;
-    if (d < a.head_dim) store_from_float(o + d, acc[i] * inv);
+    for (int i = 0; i < CH * W; ++i) {
+      const int d = (i / W) * 128 + lane * W + i % W;
+      if (d < a.head_dim) store_from_float(o + d, acc[i] * inv);
+    }
   }
 }
 

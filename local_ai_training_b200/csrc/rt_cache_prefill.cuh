@@ -44,14 +44,6 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void *gmem
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0)
                : "memory");
 }
-template <int N>
-__device__ __forceinline__ void set_registers_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void set_registers_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -72,8 +64,6 @@ struct KpShape {
   static constexpr int SMEM_USED = BAR_OFF + 256 + 1024;
   static constexpr int SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;
   static constexpr int THREADS = 16 * 32;
-  // registers per thread of the four warpgroups: 2 · 152 + 128 + 80 = 4 · 128, the launch's own
-  static constexpr int R_SOFTMAX = 152, R_REST = 80;
   static constexpr uint32_t COL_S = 0, COL_O = 256;  // + 128 (scores) or + D (outputs) for row tile B
   static constexpr uint32_t IDESC_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((KEYS >> 3) << 17) | ((ROWS >> 4) << 24);
   static constexpr uint32_t IDESC_PV =
@@ -161,7 +151,7 @@ __device__ __forceinline__ void kv_prefill_codes(const KvCache &c, const KvBatch
     }
     cp_async_wait<0>();
     uint8_t *tile = smem + (part == 0 ? SH::K_OFF : SH::V_OFF) + st * SH::TILE;
-#pragma unroll 2
+#pragma unroll 1
     for (int id = t; id < ALL; id += N) {
       const uint4 v = *reinterpret_cast<const uint4 *>(raw + id * 16);
       const int row = id / P, pcol = id % P;
@@ -230,22 +220,37 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
   };
 
   if (warp < 8) {
-    set_registers_up<SH::R_SOFTMAX>();
     // ================================================================ softmax of row tile x
     const int x = warp >> 2, r = tid & 127;  // r: row of the tile, TMEM lane
     const uint32_t t_s = tmem + SH::COL_S + x * 128 + (static_cast<uint32_t>(warp & 3) << 21);
     const uint32_t t_o = tmem + SH::COL_O + x * D + (static_cast<uint32_t>(warp & 3) << 21);
     uint32_t n_q = 0, n_s = 0, n_o = 0, n_f = 0;  // phases of q_ready, s_full, o_done; tiles of the CTA
     bool ok = true, first_piece = true;
+    constexpr int CH = D / 8, STEP = 128 / CH;  // 16-byte chunks of a row, rows of 128 chunks
+    const bool even = a.group_shift >= 0 && a.group <= STEP;  // STEP rows on: the same head
     const bool flip = a.scale_log2 < 0.0f;  // the factors are kept >= 0 (maxima): q takes the sign
     while (w.left > 0) {
       const int row0 = w.tile * SH::RT + x * SH::ROWS, all = w.q.n * a.group;
       const int rows = max(min(SH::ROWS, all - row0), 0);
       // ---- Q tile, rows beyond the unit as zeros
       {
-        constexpr int CH = D / 8;  // 16-byte chunks of a row
         uint8_t *qt = smem + SH::Q_OFF + x * SH::TILE;
-        const bool direct = a.q_vec && !flip;
+        if (a.q_vec && !flip && even) {
+          // a thread's chunks are STEP rows apart: one column, one place in the swizzle, one head
+          int token, sub;
+          kv_row(a, row0 + r / CH, token, sub);
+          const __nv_bfloat16 *first = static_cast<const __nv_bfloat16 *>(a.q), *qp =
+              first + (w.q.c0 + static_cast<int64_t>(token)) * a.q_token +
+              static_cast<int64_t>(w.head * a.group + sub) * a.q_head + r % CH * 8;
+          const uint32_t dst = smem_u32(qt + (r % CH >> 3) * SH::SUB + r / CH * 128 +
+                                        (((r % CH & 7) ^ (r / CH & 7)) << 4));
+#pragma unroll 4
+          for (int i = 0; i < CH; ++i) {
+            const bool in = r / CH + i * STEP < rows;
+            cp_async16_zfill(dst + i * STEP * 128, in ? qp : first, in);
+            qp += (STEP >> a.group_shift) * a.q_token;
+          }
+        } else {
 #pragma unroll 1
         for (int id = r; id < CH * 128; id += 128) {
           const int qr = id / CH, ch = id % CH;
@@ -256,16 +261,13 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
                                     (w.q.c0 + static_cast<int64_t>(token)) * a.q_token +
                                     static_cast<int64_t>(w.head * a.group + sub) * a.q_head + ch * 8;
           uint8_t *dst = qt + (ch >> 3) * SH::SUB + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4);
-          if (direct) {
-            cp_async16_zfill(smem_u32(dst), qp, in);
-          } else {
 #pragma unroll 1
-            for (int k = 0; k < 8; ++k) {
-              uint32_t u = in && ch * 8 + k < a.head_dim ? *reinterpret_cast<const uint16_t *>(qp + k) : 0u;
-              if (flip) u ^= 0x8000u;
-              *reinterpret_cast<uint16_t *>(dst + 2 * k) = static_cast<uint16_t>(u);
-            }
+          for (int k = 0; k < 8; ++k) {
+            uint32_t u = in && ch * 8 + k < a.head_dim ? *reinterpret_cast<const uint16_t *>(qp + k) : 0u;
+            if (flip) u ^= 0x8000u;
+            *reinterpret_cast<uint16_t *>(dst + 2 * k) = static_cast<uint16_t>(u);
           }
+        }
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -358,6 +360,8 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
           const float over = scores(known ? m : 0.0f);
           if (__any_sync(0xffffffffu, known ? over > 8.0f : over > -INFINITY)) {
             move(h, over);
+            tmem_ld_32x32b_x32(t_s + h * 32, s);  // (not kept above: registers)
+            tmem_ld_wait_regs(s);
             scores(m > -1e30f ? m : 0.0f);
           }
           uint32_t p[16];
@@ -408,7 +412,6 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
         const int parts = whole ? 1 : 2;
 #pragma unroll 1
         for (int part = 0; part < parts; ++part) {
-          constexpr int PIECES = D / 8;  // 16-byte pieces of a staged row
           const int c0 = part * (D / 2), n32 = whole ? D / 32 : D / 64;
 #pragma unroll 1
           for (int h = 0; h < n32; ++h) {
@@ -427,26 +430,43 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   u[k] = pack_bf16x2(__uint_as_float(o[i + 2 * k]) * scale, __uint_as_float(o[i + 2 * k + 1]) * scale);
-                *reinterpret_cast<uint4 *>(stage + (r * PIECES + ((h * 4 + i / 8) ^ (r & 7))) * 16) =
+                *reinterpret_cast<uint4 *>(stage + (r * CH + ((h * 4 + i / 8) ^ (r & 7))) * 16) =
                     make_uint4(u[0], u[1], u[2], u[3]);
               }
             } else {
 #pragma unroll
               for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4 *>(stage + (r * PIECES + ((h * 8 + i / 4) ^ (r & 7))) * 16) =
+                *reinterpret_cast<uint4 *>(stage + (r * CH + ((h * 8 + i / 4) ^ (r & 7))) * 16) =
                     make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
           }
           warpgroup_and(1 + x, true);
-#pragma unroll 1
-          for (int id = r; id < PIECES * 128; id += 128) {
-            const int sr = id / PIECES, pc = id % PIECES;
-            const uint4 v = *reinterpret_cast<const uint4 *>(stage + (sr * PIECES + (pc ^ (sr & 7))) * 16);
-            if (!whole) {
-              if (sr < rows)
-                *reinterpret_cast<uint4 *>(ws + static_cast<int64_t>(sr) * (D + 4) + 4 + c0 + pc * 4) = v;
-              continue;
+          const uint8_t *mine = stage + (r / CH * CH + (r % CH ^ (r / CH & 7))) * 16;
+          if (!whole || (a.o_vec && even)) {
+            int token, sub;
+            kv_row(a, row0 + r / CH, token, sub);
+            uint8_t *at;
+            int64_t step;
+            if (whole) {
+              at = reinterpret_cast<uint8_t *>(static_cast<__nv_bfloat16 *>(a.out) +
+                                               (w.q.c0 + static_cast<int64_t>(token)) * a.o_token +
+                                               static_cast<int64_t>(w.head * a.group + sub) * a.o_head + r % CH * 8);
+              step = (STEP >> a.group_shift) * a.o_token * 2;
+            } else {
+              at = reinterpret_cast<uint8_t *>(ws + static_cast<int64_t>(r / CH) * (D + 4) + 4 + c0 + r % CH * 4);
+              step = STEP * (D + 4) * 4;
             }
+#pragma unroll 4
+            for (int i = 0; i < CH; ++i) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(mine + i * 2048);
+              if (r / CH + i * STEP < rows) *reinterpret_cast<uint4 *>(at) = v;
+              at += step;
+            }
+          } else {
+#pragma unroll 1
+          for (int id = r; id < CH * 128; id += 128) {
+            const int sr = id / CH, pc = id % CH;
+            const uint4 v = *reinterpret_cast<const uint4 *>(stage + (sr * CH + (pc ^ (sr & 7))) * 16);
             int token, sub;
             kv_row(a, row0 + sr, token, sub);
             __nv_bfloat16 *op = static_cast<__nv_bfloat16 *>(a.out) +
@@ -461,6 +481,7 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
                 if (sr < rows && pc * 8 + k < a.head_dim)
                   *reinterpret_cast<uint16_t *>(op + pc * 8 + k) = static_cast<uint16_t>(u[k >> 1] >> (k & 1) * 16);
             }
+          }
           }
           warpgroup_and(1 + x, true);
         }
@@ -480,7 +501,6 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
   } else if (warp < 12) {
     kv_prefill_codes<D, 0, 128>(c, bt, a, w, smem, bar, tid - 256);
   } else {
-    set_registers_down<SH::R_REST>();
     if (warp < 15) {
       kv_prefill_codes<D, 1, 96>(c, bt, a, w, smem, bar, tid - 384);
     } else if (lane == 0) {
