@@ -397,7 +397,8 @@ int rt_token_windows(const uint16_t *data, int64_t n, const int64_t *starts, int
  * rt_kv_attention: out[t, h] = softmax over the keys at positions <= row t's own of
  *   softmax_scale * (q[t, h] . k), times v; query head h reads kv head h / (q_heads / kv_heads).
  *   A row that sees no key is zero.  Scores, maxima, sums and outputs are fp32, rounded once to dtype.
- *   workspace: rt_kv_attention_workspace_bytes(...) bytes, 256-byte aligned, no initial contents.
+ *   workspace: rt_kv_attention_workspace_bytes(...) bytes (0: none), 256-byte aligned, no initial
+ *   contents.
  * ------------------------------------------------------------------------------------------- */
 int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t kv_heads, int64_t page_size,
                  int64_t padded_dim, const int32_t *page_table, int64_t pages_per_seq,
@@ -420,7 +421,8 @@ int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token, int64_t q_
                     void *out, int64_t o_stride_token, int64_t o_stride_head, void *workspace,
                     int64_t workspace_bytes, void *stream);
 int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
-                                        int64_t kv_heads, int64_t padded_dim);
+                                        int64_t kv_heads, int64_t padded_dim, int64_t page_size,
+                                        int64_t pages_per_seq, int dtype);
 
 #ifdef __cplusplus
 }

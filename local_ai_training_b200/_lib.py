@@ -95,7 +95,7 @@ _SIGNATURES = {
     "rt_kv_copy_pages": ([_p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p], _i),
     "rt_kv_attention": ([_p, _i, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i64,
                          _p, _p, _i64, _i64, _d, _p, _i64, _i64, _p, _i64, _p], _i),
-    "rt_kv_attention_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64], _i64),
+    "rt_kv_attention_workspace_bytes": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i], _i64),
 }
 
 

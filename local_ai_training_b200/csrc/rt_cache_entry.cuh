@@ -43,27 +43,35 @@ inline int kv_allow_smem(K *kernel, int bytes, std::mutex &mu, bool (&done)[64])
 
 // Row tiles of a batch, at most: a partly filled one per sequence with rows, and one per token while a
 // token's rows fit a tile.
-inline int64_t kv_most_tiles(const KvBatch &bt, int group, int tile) {
-  const int64_t some = std::min(bt.n_tokens, bt.n_seqs);
-  const int64_t tiles = (bt.n_tokens * group + some * (tile - 1)) / tile;
-  return group <= tile ? std::min(tiles, bt.n_tokens) : tiles;
+inline int64_t kv_most_tiles(int64_t n_seqs, int64_t n_tokens, int64_t group, int tile) {
+  const int64_t tiles = (n_tokens * group + std::min(n_tokens, n_seqs) * (tile - 1)) / tile;
+  return group <= tile ? std::min(tiles, n_tokens) : tiles;
+}
+// Rows of a tile of the few-row kernels, by the rows that the sequences average per kv head.
+inline int kv_tile(int64_t n_seqs, int64_t n_tokens, int64_t group, int64_t dim) {
+  const int64_t rows = n_tokens * group;
+  if (dim == 128) return rows > 4 * n_seqs ? 16 : 4;
+  return dim < 128 && rows > 8 * n_seqs ? 16 : 8;
 }
 // Few and short units take one CTA each and no join, whose launch would cost more than the few tokens that a
-// CTA then takes: at most `shortest`.  Returns their number, or 0 when the line is to be cut.
-inline int64_t kv_whole_units(const KvCache &c, const KvBatch &bt, const KvAttn &a, int tile, int ctas, int shortest) {
-  const int64_t units = kv_most_tiles(bt, a.group, tile) * c.kv_heads;
-  return units <= ctas && bt.pages_per_seq * c.page_size <= shortest ? units : 0;
+// CTA then takes.  Returns their number, or 0 when the line is to be cut.
+inline int64_t kv_whole_units(int64_t n_seqs, int64_t n_tokens, int64_t group, int64_t kv_heads, int64_t dim,
+                              int64_t room, int dtype, int64_t sms) {
+  const int tile = kv_tile(n_seqs, n_tokens, group, dim);
+  const int64_t ctas = sms * (dim == 128 || (dim < 128 && tile == 8 && dtype == RT_BF16) ? 2 : 1);
+  const int64_t units = kv_most_tiles(n_seqs, n_tokens, group, tile) * kv_heads;
+  return units <= (room <= 512 && dim < 128 ? 2 * ctas : ctas) && room <= (dim == 128 ? 512 : 1024) ? units : 0;
 }
 
 template <typename T, int D, int NT>
-int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, int64_t units, cudaStream_t s) {
   using SH = KaShape<T, D, NT>;
   static std::mutex mu;
   static bool done[64] = {false};
   auto *kernel = kv_attention_kernel<T, D, NT>;
   if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
   const int ctas = sms * SH::MIN_CTAS;
-  if (const int64_t units = kv_whole_units(c, bt, a, SH::RT, ctas, 1024)) {
+  if (units > 0) {
     launch_k(kernel, static_cast<unsigned>(units), KA_WARPS * 32, SH::SMEM, s, c, bt, a, 0);
     return check_launch("kv_attention");
   }
@@ -72,7 +80,7 @@ int kv_attention_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int s
   return check_launch("kv_attention");
 }
 template <typename T, int RT>
-int kv_decode_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
+int kv_decode_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, int64_t units, cudaStream_t s) {
   using SH = KdShape<T, RT>;
   static std::mutex mu;
   static bool done[64] = {false};
@@ -85,7 +93,7 @@ int kv_decode_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms,
                         std::min(c.page_size, SH::KEYS)))
     return rc;
   const int ctas = sms * SH::CTAS;
-  if (const int64_t units = kv_whole_units(c, bt, a, RT, ctas, 512)) {
+  if (units > 0) {
     launch_k(kernel, static_cast<unsigned>(units), SH::THREADS, SH::SMEM, s, map, c, bt, a, 0);
     return check_launch("kv_attention");
   }
@@ -105,19 +113,19 @@ int kv_prefill_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms
   return check_launch("kv_attention");
 }
 template <typename T>
-int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, cudaStream_t s) {
-  // row tiles by the rows that the sequences average per kv head
-  const int64_t rows = bt.n_tokens * a.group;
-  const bool wide = rows > 8 * bt.n_seqs;
+int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms, int64_t units, cudaStream_t s) {
+  const bool wide = kv_tile(bt.n_seqs, bt.n_tokens, a.group, c.dim) == 16;
   switch (c.dim) {
     case 32:
-      return wide ? kv_attention_run<T, 32, 2>(c, bt, a, sms, s) : kv_attention_run<T, 32, 1>(c, bt, a, sms, s);
+      return wide ? kv_attention_run<T, 32, 2>(c, bt, a, sms, units, s)
+                  : kv_attention_run<T, 32, 1>(c, bt, a, sms, units, s);
     case 64:
-      return wide ? kv_attention_run<T, 64, 2>(c, bt, a, sms, s) : kv_attention_run<T, 64, 1>(c, bt, a, sms, s);
+      return wide ? kv_attention_run<T, 64, 2>(c, bt, a, sms, units, s)
+                  : kv_attention_run<T, 64, 1>(c, bt, a, sms, units, s);
     case 128:
-      return rows > 4 * bt.n_seqs ? kv_decode_run<T, 16>(c, bt, a, sms, s) : kv_decode_run<T, 4>(c, bt, a, sms, s);
+      return wide ? kv_decode_run<T, 16>(c, bt, a, sms, units, s) : kv_decode_run<T, 4>(c, bt, a, sms, units, s);
     default:
-      return kv_attention_run<T, 256, 1>(c, bt, a, sms, s);
+      return kv_attention_run<T, 256, 1>(c, bt, a, sms, units, s);
   }
 }
 
@@ -126,11 +134,15 @@ int kv_attention_width(const KvCache &c, const KvBatch &bt, const KvAttn &a, int
 using namespace rt;
 
 extern "C" int64_t rt_kv_attention_workspace_bytes(int64_t n_seqs, int64_t n_tokens, int64_t q_heads,
-                                                   int64_t kv_heads, int64_t padded_dim) {
+                                                   int64_t kv_heads, int64_t padded_dim,
+                                                   int64_t page_size, int64_t pages_per_seq, int dtype) {
   if (kv_heads <= 0 || n_tokens <= 0) return 0;
   const int64_t sms = kv_sm_count();
-  return kv_few_bytes(sms, padded_dim) +
-         (kv_prefill_fits(n_seqs, n_tokens, q_heads, kv_heads, padded_dim) ? kv_prefill_bytes(sms, padded_dim) : 0);
+  if (dtype == RT_BF16 && kv_prefill_fits(n_seqs, n_tokens, q_heads, kv_heads, padded_dim))
+    return kv_few_bytes(sms, padded_dim) + kv_prefill_bytes(sms, padded_dim);
+  const int64_t units = kv_whole_units(n_seqs, n_tokens, q_heads / kv_heads, kv_heads, padded_dim,
+                                       pages_per_seq * page_size, dtype, sms);
+  return units > 0 ? 0 : kv_few_bytes(sms, padded_dim);
 }
 
 extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
@@ -166,8 +178,9 @@ extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
     return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
   const int sms = kv_sm_count();
   if (sms <= 0) return fail(RT_ERR_CUDA, "kv_attention: no device");
-  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
-      workspace_bytes < rt_kv_attention_workspace_bytes(n_seqs, n_tokens, q_heads, kv_heads, padded_dim))
+  const int64_t need = rt_kv_attention_workspace_bytes(n_seqs, n_tokens, q_heads, kv_heads, padded_dim, page_size,
+                                                       pages_per_seq, dtype);
+  if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 || workspace_bytes < need))
     return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: workspace too small or not 256-byte aligned");
   KvAttn a{};
   a.q = q, a.q_token = q_stride_token, a.q_head = q_stride_head;
@@ -202,6 +215,9 @@ extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
   }
   a.meta = reinterpret_cast<int4 *>(ws);
   a.ws = reinterpret_cast<float *>(ws + sms * KA_GRID * 16);
-  return dtype == RT_F32 ? kv_attention_width<float>(c, b, a, sms, s)
-                         : kv_attention_width<__nv_bfloat16>(c, b, a, sms, s);
+  const int64_t units = prefill ? 0
+                                : kv_whole_units(n_seqs, n_tokens, a.group, kv_heads, padded_dim,
+                                                 pages_per_seq * page_size, dtype, sms);
+  return dtype == RT_F32 ? kv_attention_width<float>(c, b, a, sms, units, s)
+                         : kv_attention_width<__nv_bfloat16>(c, b, a, sms, units, s);
 }

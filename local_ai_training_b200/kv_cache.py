@@ -72,8 +72,10 @@ def _check_batch(page_table: Tensor, lens: Tensor, cu_tokens: Tensor, what: str)
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_workspace(seqs: int, tokens: int, heads: int, kv_heads: int, width: int, device: int) -> int:
-    return _lib.lib().rt_kv_attention_workspace_bytes(seqs, tokens, heads, kv_heads, width)
+def _attention_workspace(seqs: int, tokens: int, heads: int, kv_heads: int, width: int, page_size: int,
+                         per_seq: int, dtype: int, device: int) -> int:
+    return _lib.lib().rt_kv_attention_workspace_bytes(seqs, tokens, heads, kv_heads, width, page_size,
+                                                      per_seq, dtype)
 
 
 def kv_append(codes: Tensor, scales: Tensor, page_table: Tensor, kv_lens: Tensor, cu_tokens: Tensor,
@@ -122,14 +124,15 @@ def kv_read(codes: Tensor, scales: Tensor, page_table: Tensor, starts: Tensor, c
         raise ValueError("kv_read: tokens must be >= 0 and head_dim in [1, stored width]")
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("kv_read: dtype must be float32 or bfloat16")
-    out = torch.empty((2, tokens, heads, head_dim), device=codes.device, dtype=dtype)
-    k, v = out.unbind(0)
-    ev = _lib.prof_start(out)
+    device = codes.device
+    k = torch.empty((tokens, heads, head_dim), device=device, dtype=dtype)
+    v = torch.empty_like(k)
+    ev = _lib.prof_start(k)
     _lib.check(_lib.lib().rt_kv_read(
         codes.data_ptr(), scales.data_ptr(), pages, heads, page_size, width, page_table.data_ptr(),
-        per_seq, starts.data_ptr(), cu_tokens.data_ptr(), seqs, tokens, head_dim, k.data_ptr(), v.data_ptr(), _lib.dtype_code(out), _lib.stream_of(codes)))
+        per_seq, starts.data_ptr(), cu_tokens.data_ptr(), seqs, tokens, head_dim, k.data_ptr(), v.data_ptr(), _lib.dtype_code(k), _lib.stream_of(codes)))
     if ev is not None:
-        _lib.prof_stop(ev, "kv_read", out, 0.0, out.numel() * (out.element_size() + 1))
+        _lib.prof_stop(ev, "kv_read", k, 0.0, 2 * k.numel() * (k.element_size() + 1))
     return k, v
 
 
@@ -194,15 +197,17 @@ def kv_attention(q: Tensor, codes: Tensor, scales: Tensor, page_table: Tensor, k
         ot, oh, _ = out.stride()
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(head_dim)
-    nbytes = _attention_workspace(seqs, tokens, heads, kv_heads, width, device.index)
+    kind = _lib.F32 if dtype is torch.float32 else _lib.BF16
+    nbytes = _attention_workspace(seqs, tokens, heads, kv_heads, width, page_size, per_seq, kind,
+                                  device.index)
     # allocated per call: the caching allocator keeps calls on different streams apart
-    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
     ev = _lib.prof_start(q)
     _lib.check(_lib.lib().rt_kv_attention(
-        q.data_ptr(), _lib.F32 if dtype is torch.float32 else _lib.BF16, qt, qh, heads, head_dim,
+        q.data_ptr(), kind, qt, qh, heads, head_dim,
         codes.data_ptr(), scales.data_ptr(), pages, kv_heads, page_size, width, page_table.data_ptr(),
         per_seq, kv_lens.data_ptr(), cu_tokens.data_ptr(), seqs, tokens, softmax_scale, out.data_ptr(),
-        ot, oh, ws.data_ptr(), nbytes, _lib.stream_of(q)))
+        ot, oh, _lib.ptr(ws), nbytes, _lib.stream_of(q)))
     if ev is not None:
         # the lengths are on the device: only the rows' own bytes are counted here
         _lib.prof_stop(ev, "kv_attention", q, 0.0, 2 * q.numel() * q.element_size())
