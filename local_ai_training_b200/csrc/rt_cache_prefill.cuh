@@ -70,9 +70,9 @@ struct KpShape {
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((D >> 3) << 17) | ((ROWS >> 4) << 24);
 };
 struct KpBars {
-  uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], f_full[4], s_full[2], p_ready[2], o_done[2];
+  uint64_t piece_ready[2], q_ready[2], k_full[2], k_empty[2], v_full[2], v_empty[2], f_full[4], s_full[2], p_ready[2], o_done[2];
   uint32_t tmem;
-  int piece[4];  // the piece's tiles: first, end, ends of row tiles A and B
+  int piece[2][4];  // the piece's tiles: first, end, ends of row tiles A and B (two pieces in turn)
 };
 static_assert(sizeof(KpBars) <= 256, "KpBars");
 struct KpFactors {  // one tile's block factors
@@ -85,8 +85,8 @@ __device__ __forceinline__ uint2 bf16x4_of_bytes(uint32_t w) {
   return make_uint2(bf16x2_of_bytes<false>(w), bf16x2_of_bytes<true>(w));
 }
 
-// Codes -> bf16 tiles: K (part 0, 128 threads) or V (part 1, 96 threads).  Thread t takes the 16-byte pieces t, t + N, ... of a
-// tile's codes, which come a tile ahead into its own slots (no barrier).  Lane i % 8 looks up block i's
+// Codes -> bf16 tiles: K (part 0, 128 threads) or V (part 1, 96 threads).  Thread t takes the 16-byte
+// pieces t, t + N, ... of a tile's codes, which come a tile ahead into its own slots (no barrier).  Lane i % 8 looks up block i's
 // page, a tile before it is used.
 template <int D, int part, int N>
 __device__ __forceinline__ void kv_prefill_codes(const KvCache &c, const KvBatch &bt, const KvAttn &a,
@@ -183,8 +183,8 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
   KpBars *bar = reinterpret_cast<KpBars *>(smem + SH::BAR_OFF);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
-    mbar_init(&bar->q_ready, 256);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->piece_ready[i], 1), mbar_init(&bar->q_ready[i], 128);
       mbar_init(&bar->k_full[i], 128), mbar_init(&bar->k_empty[i], 1);
       mbar_init(&bar->v_full[i], 96), mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 1), mbar_init(&bar->p_ready[i], 128), mbar_init(&bar->o_done[i], 1);
@@ -224,16 +224,25 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
     const int x = warp >> 2, r = tid & 127;  // r: row of the tile, TMEM lane
     const uint32_t t_s = tmem + SH::COL_S + x * 128 + (static_cast<uint32_t>(warp & 3) << 21);
     const uint32_t t_o = tmem + SH::COL_O + x * D + (static_cast<uint32_t>(warp & 3) << 21);
-    uint32_t n_q = 0, n_s = 0, n_o = 0, n_f = 0;  // phases of q_ready, s_full, o_done; tiles of the CTA
-    bool ok = true, first_piece = true;
+    uint32_t pieces = 0, n_s = 0, n_o = 0, n_f = 0;  // phases of s_full, o_done; tiles of the CTA
+    bool ok = true;
     constexpr int CH = D / 8, STEP = 128 / CH;  // 16-byte chunks of a row, rows of 128 chunks
     const bool even = a.group_shift >= 0 && a.group <= STEP;  // STEP rows on: the same head
     const bool flip = a.scale_log2 < 0.0f;  // the factors are kept >= 0 (maxima): q takes the sign
     while (w.left > 0) {
       const int row0 = w.tile * SH::RT + x * SH::ROWS, all = w.q.n * a.group;
       const int rows = max(min(SH::ROWS, all - row0), 0);
-      // ---- Q tile, rows beyond the unit as zeros
-      {
+      const int end = tiles_of(x);
+      if (tid == 0) {
+        // (of two pieces at most one lies ahead of the products: only a CTA's first can have none for A)
+        int *info = bar->piece[pieces & 1];
+        info[0] = w.b, info[1] = w.e, info[2] = end, info[3] = tiles_of(1);
+        mbar_arrive(&bar->piece_ready[pieces & 1]);
+      }
+      ++pieces;
+      // ---- Q tile, rows beyond the unit as zeros.  The row tiles are apart: one's products begin while the
+      // other still writes its rows of the piece before.
+      if (end > w.b) {
         uint8_t *qt = smem + SH::Q_OFF + x * SH::TILE;
         if (a.q_vec && !flip && even) {
           // a thread's chunks are STEP rows apart: one column, one place in the swizzle, one head
@@ -271,23 +280,19 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
         }
         cp_async_commit();
         cp_async_wait<0>();
-        if (tid == 0) bar->piece[0] = w.b, bar->piece[1] = w.e, bar->piece[2] = tiles_of(0), bar->piece[3] = tiles_of(1);
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(&bar->q_ready);
-        // (also keeps a row tile without rows from running a piece ahead of the other)
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->q_ready, n_q & 1));
-        ++n_q;
+        mbar_arrive(&bar->q_ready[x]);
       }
-      const int end = tiles_of(x);
       const int tok = (row0 + min(r, max(rows - 1, 0))) / a.group;
       const int lim = min(w.q.start + tok + 1, w.q.len);  // keys this row sees
       float m = -1e30f;
       float2 l2 = make_float2(0.0f, 0.0f);  // sum of weights, even and odd keys
       for (int j = w.b; j < end && ok; ++j) {
         const uint32_t f_at = n_f + static_cast<uint32_t>(j - w.b);
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->f_full[f_at & 3], (f_at >> 2) & 1) &&
-                                         mbar_wait(&bar->s_full[x], n_s & 1));
+        // (the scores first: a row tile that had no part in the pieces before is then not ahead of the factors)
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[x], n_s & 1) &&
+                                         mbar_wait(&bar->f_full[f_at & 3], (f_at >> 2) & 1));
         if (!ok) break;
         ++n_s;
         tc_fence_after();
@@ -489,11 +494,10 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
       }
       if (tid == 0) {
         int4 *mt = a.meta + blockIdx.x;
-        if (first_piece) *mt = make_int4(-1, 0, 0, 0);
+        if (pieces == 1) *mt = make_int4(-1, 0, 0, 0);
         if (w.b > 0) mt->w = w.e == w.nb;
         if (w.b == 0 && !whole) mt->x = w.s, mt->y = w.tile, mt->z = w.head;
       }
-      first_piece = false;
       n_f += static_cast<uint32_t>(w.e - w.b);
       if (!ok) break;
       w.next(c, bt, a);
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
     } else if (lane == 0) {
     // ================================================================ MMA issue
     const uint32_t q0 = smem_u32(smem + SH::Q_OFF), k0 = smem_u32(smem + SH::K_OFF), v0 = smem_u32(smem + SH::V_OFF);
-    uint32_t n = 0, n_q = 0, n_p[2] = {0, 0};
+    uint32_t n = 0, pieces = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
     bool ok = true;
     const auto qk = [&](int x, uint32_t tile) {
       tc_fence_after();
@@ -531,13 +535,19 @@ __global__ void __launch_bounds__(KpShape<D>::THREADS, 1)
     };
     const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
     while (n < total && ok) {
-      ok = mbar_wait(&bar->q_ready, n_q & 1) && mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1);
-      ++n_q;
+      ok = mbar_wait(&bar->piece_ready[pieces & 1], (pieces >> 1) & 1) && mbar_wait(&bar->k_full[n & 1], (n >> 1) & 1);
       if (!ok) break;
-      const int b = bar->piece[0], e = bar->piece[1], end[2] = {bar->piece[2], bar->piece[3]};
+      const int *info = bar->piece[pieces & 1];
+      const int b = info[0], e = info[1], end[2] = {info[2], info[3]};
+      ++pieces;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        if (end[x] > b) qk(x, n);
+        if (ok && end[x] > b) {
+          ok = mbar_wait(&bar->q_ready[x], n_q[x] & 1);
+          ++n_q[x];
+          if (ok) qk(x, n);
+        }
+      if (!ok) break;
       umma_commit(&bar->k_empty[n & 1]);
       for (int j = b; j < e && ok; ++j, ++n) {
         ok = mbar_wait(&bar->v_full[n & 1], (n >> 1) & 1);

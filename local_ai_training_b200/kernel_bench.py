@@ -296,12 +296,46 @@ def bench_unpack(rows, cols, reps, flush, peaks):
     return _report("unpack_codes", [rows, cols], t, 2 * rows * cols, 0, 0, peaks)
 
 
+def bench_cache(which, seqs, tokens, new, heads, kv_heads, reps, flush, peaks, layers=1):
+    """The key/value cache: `decode` / `prefill` attention of the `new` newest of `tokens` tokens of each of
+    `seqs` sequences (heads of 128, bf16, 64-token pages), `append` of the `new` newest, `copy` of the
+    pages of `seqs` sequences over `layers` layers."""
+    from . import kv_cache
+
+    dev = torch.device("cuda")
+    per = -(-tokens // 64)
+    pages = seqs * per * (2 if which == "copy" else 1)
+    codes = torch.randint(-127, 128, (layers, pages, 2, kv_heads, 64, 128), device=dev, dtype=torch.int8)
+    scales = torch.rand(layers, pages, 2, kv_heads, 4, device=dev) * 0.01 + 0.02
+    order = torch.randperm(pages, device=dev).to(torch.int32)
+    if which == "copy":
+        half = seqs * per
+        t = _time(lambda: kv_cache.kv_copy_pages(codes, scales, order[:half], order[half:]), reps, flush)
+        nbytes = 2 * layers * half * 2 * kv_heads * 64 * (128 + 0.25)
+        return _report("kv_copy_pages", [layers, half, kv_heads], t, nbytes, 0, 0, peaks)
+    table = order.view(seqs, per)
+    lens = torch.full((seqs,), tokens, device=dev, dtype=torch.int32)
+    cu = torch.arange(seqs + 1, device=dev, dtype=torch.int32) * new
+    if which == "append":
+        qkv = torch.randn(seqs * new, 3 * kv_heads * 128, device=dev).to(torch.bfloat16)
+        k, v = (part.view(-1, kv_heads, 128) for part in qkv.chunk(3, dim=-1)[1:])
+        t = _time(lambda: kv_cache.kv_append(codes[0], scales[0], table, lens, cu, k, v), reps, flush)
+        return _report("kv_append", [seqs, new, kv_heads], t, 3 * k.numel() * 2, 0, 0, peaks)
+    q = torch.randn(seqs * new, heads, 128, device=dev).to(torch.bfloat16)
+    t = _time(lambda: kv_cache.kv_attention(q, codes[0], scales[0], table, lens, cu), reps, flush)
+    seen = seqs * (new * tokens - new * (new - 1) // 2)
+    nbytes = seqs * tokens * kv_heads * 256.5 + 4 * q.numel()
+    return _report(f"kv_attention_{which}", [seqs, tokens, new, heads, kv_heads], t, nbytes,
+                   4.0 * seen * heads * 128, peaks["bf16_tflops"], peaks)
+
+
 def main() -> None:
     parser = argparse.ArgumentParser()
     parser.add_argument("kernel", choices=["all", "all1b", "fwd", "grad_input", "gradw", "quant_sr",
                                            "quant_rn", "dequant", "update", "update_grouped",
                                            "rmsnorm_bwd", "producers", "gelu_bwd", "ce",
-                                           "matmul_bf16", "unpack"])
+                                           "matmul_bf16", "unpack", "cache", "cache_decode",
+                                           "cache_prefill", "cache_append", "cache_copy"])
     parser.add_argument("--m", type=int, default=16384)
     parser.add_argument("--k", type=int, default=512)
     parser.add_argument("--n", type=int, default=2048)
@@ -381,6 +415,18 @@ def main() -> None:
         bench_matmul_bf16(m, args.k, args.n, args.reps, flush, peaks)
     elif args.kernel == "unpack":
         bench_unpack(args.n, args.k, args.reps, flush, peaks)
+    if args.kernel in ("cache", "cache_decode"):
+        bench_cache("decode", 64, 1024, 1, 16, 16, args.reps, flush, peaks)
+    if args.kernel == "cache":
+        bench_cache("decode", 16, 32768, 1, 32, 8, args.reps, flush, peaks)
+        bench_cache("decode", 32, 4096, 4, 32, 8, args.reps, flush, peaks)
+    if args.kernel in ("cache", "cache_prefill"):
+        bench_cache("prefill", 8, 1024, 1024, 16, 16, args.reps, flush, peaks)
+        bench_cache("prefill", 1, 8192, 2048, 32, 8, args.reps, flush, peaks)
+    if args.kernel in ("cache", "cache_append"):
+        bench_cache("append", 16, 1024, 1024, 16, 16, args.reps, flush, peaks)
+    if args.kernel in ("cache", "cache_copy"):
+        bench_cache("copy", 3, 1024, 0, 16, 16, args.reps, flush, peaks, layers=20)
 
 
 if __name__ == "__main__":
