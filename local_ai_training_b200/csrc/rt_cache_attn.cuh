@@ -1,6 +1,7 @@
 // rt_cache_attn.cuh — causal attention of a batch's newest tokens over the paged int8 cache
-// (rt_cache.cuh), for few query rows per key/value head: single tokens, drafted tokens, and every
-// type and width.
+// (rt_cache.cuh), for few query rows per key/value head (single tokens, drafted tokens) and every type,
+// at heads of other widths than 128.  What it shares with the other kernels: the line of work
+// (KvWalk, kv_walk_start) and the joining of cut units.
 //
 // Mathematics.  For a query row r (token position p, query head of kv head h) and the keys j <= p:
 //   t_j = (softmax_scale · log2 e · sk_b) (q_r · K_j)   K_j int8 codes, sk_b, sv_b the scales of j's block
@@ -19,6 +20,9 @@
 //   P^T's operand is S^T's accumulator transposed within the warp (movmatrix).
 // Each lane copies exactly the bytes it will use (cp.async, its own slots), so a warp's ring of
 // stages needs no barrier.
+//
+// Bound by the conversion of the codes, some two instructions each, next to one byte of HBM: 64 sequences of
+// 1024 tokens, 8 heads of 64, run in 33 us (2.0 TB/s); one of 512 in 8.2 us, most of it launch and latency.
 //
 // Work split: the key blocks of all (sequence, row tile, kv head) units are one line, cut into equal
 // pieces, one per CTA; the eight warps of a CTA take its blocks in turn and merge in shared memory.
@@ -167,13 +171,13 @@ struct KvWalk {
 };
 
 // Sets this CTA's share of the line: all of the grid has equal shares of a long line, and as many CTAs as
-// get min_blocks each of a short one.  With min_blocks = 0 a CTA takes one whole unit (the grid has one
+// get min_blocks each of a short one; `used`: the batch's rows.  With min_blocks = 0 a CTA takes one whole unit (the grid has one
 // for each), so no rows are left to join.  Returns false (for every thread) when this CTA has no share.
 template <int THREADS, int RT, int KEYS>
 __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache &c, const KvBatch &bt,
-                                              const KvAttn &a, int min_blocks) {
+                                              const KvAttn &a, int min_blocks, int &used) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ int sm_sum[WARPS], sm_start[5];
+  __shared__ int sm_sum[WARPS], sm_start[10];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool units = min_blocks == 0;
   // a thread's sequences (one each, up to THREADS of them); the line's length fits 31 bits (host check)
@@ -191,7 +195,9 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
   }
   if (lane == 31) sm_sum[warp] = scan;
   if (tid == 0) sm_start[0] = -1;
+  if (s1 == seqs && (s0 < s1 || (seqs == 0 && tid == 0))) sm_start[9] = seqs == 0 ? 0 : w.q.c0 + w.q.n;
   __syncthreads();
+  used = sm_start[9];
   int before = scan - mine, total = 0;
 #pragma unroll
   for (int i = 0; i < WARPS; ++i) {
@@ -214,7 +220,7 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
         at += n;
         ++w.s;
       }
-      w.set_seq(c, bt, a);
+      if (per > 1) w.set_seq(c, bt, a);  // (else it is at hand)
       int per_head;
 #pragma unroll 1
       for (w.tile = 0;; ++w.tile) {
@@ -225,23 +231,23 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
       }
       sm_start[0] = w.s, sm_start[1] = w.tile, sm_start[2] = (p0 - at) / per_head;
       sm_start[3] = p0 - at - sm_start[2] * per_head, sm_start[4] = units ? w.nb : p1 - p0;
+      sm_start[5] = w.q.c0, sm_start[6] = w.q.n, sm_start[7] = w.q.len, sm_start[8] = w.tiles;
     }
   }
   __syncthreads();
   if (sm_start[0] < 0) return false;
   w.s = sm_start[0], w.tile = sm_start[1], w.head = sm_start[2], w.b = sm_start[3];
   w.left = sm_start[4];
-  w.set_seq(c, bt, a);
+  w.q = KvSeq{sm_start[5], sm_start[6], sm_start[7], sm_start[7] - sm_start[6]};
+  w.tiles = sm_start[8];
   w.set_tile(a);
   w.e = min(w.nb, w.b + w.left);
   return true;
 }
 
-// Zeros for the rows that belong to no sequence (from cu[n_seqs] on).
+// Zeros for the rows that belong to no sequence (from cu[n_seqs] = used on).
 template <typename T>
-__device__ __forceinline__ void kv_zero_rest(const KvBatch &bt, const KvAttn &a) {
-  const int64_t end = bt.n_seqs > 0 ? bt.cu[bt.n_seqs] : 0;
-  const int64_t first = max(min(end, bt.n_tokens), static_cast<int64_t>(0));
+__device__ __forceinline__ void kv_zero_rest(const KvBatch &bt, const KvAttn &a, int64_t first) {
   const int64_t n = (bt.n_tokens - first) * a.q_heads * a.head_dim;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -282,9 +288,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
   pdl_wait();
   pdl_trigger();
 
-  kv_zero_rest<T>(bt, a);
   KvWalk<RT, KV_BLOCK> w;
-  if (!kv_walk_start<KA_WARPS * 32>(w, c, bt, a, min_blocks)) {
+  int used;
+  const bool busy = kv_walk_start<KA_WARPS * 32>(w, c, bt, a, min_blocks, used);
+  kv_zero_rest<T>(bt, a, used);
+  if (!busy) {
     if (tid == 0 && min_blocks != 0) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }

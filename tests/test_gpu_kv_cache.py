@@ -258,6 +258,32 @@ def test_attention_zero_and_tiny_blocks(cuda_device, dtype, news):
     case.check(case.run(q), q)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("news", [[1, 3], [150, 3]])
+def test_attention_nan_query_stays_in_its_row(cuda_device, dim, news, dtype):
+    case = _Case(cuda_device, [300, 50], news, heads=4, kv_heads=2, dim=dim)
+    q = case.queries(dtype)
+    first = case.run(q)
+    q[news[0], 2, 5] = float("nan")
+    out = case.run(q)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[news[0], 2] = True
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], first[~hit])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [64, 95, 96, 97, 127, 128, 129, 255, 256, 257])
+def test_attention_rows_around_the_tiles(cuda_device, rows, dim):
+    """Row counts on both sides of the kernels' choice and of their row tiles, alone and next to others."""
+    for lens, news in (([rows + 37], [rows]), ([rows, 64, rows + 600], [rows, 1, rows])):
+        case = _Case(cuda_device, lens, news, heads=2, kv_heads=2, dim=dim, page=16, seed=rows)
+        q = case.queries(torch.bfloat16)
+        case.check(case.run(q), q)
+    assert _status(cuda_device) == 0
+
+
 def test_attention_bad_pages_and_lengths_are_flagged(cuda_device):
     case = _Case(cuda_device, [60, 60], [1, 1])
     q = case.queries(torch.bfloat16)
