@@ -148,7 +148,7 @@ struct KvPiece {
   int in_page, p0, p1;
   int piece, stride;  // K's heads, then V's
 };
-__device__ __forceinline__ bool kv_append_piece(const KvCache &c, const KvBatch &b, int slots, KvPiece &x) {
+__device__ __forceinline__ bool kv_append_piece(const KvCache &c, const KvBatch &b, KvPiece &x) {
   const int slot = blockIdx.x;
   const int64_t s = kv_warp_search(b.n_seqs, slot, [&](int64_t i) {
     return static_cast<int64_t>(max(__ldg(b.cu + i), 0) >> 4) + 2 * i;
@@ -173,12 +173,12 @@ __device__ __forceinline__ int8_t kv_code(float v, float s) {
 
 // Any strides and widths: the rows are read twice, the second time from the cache.
 template <typename T>
-__global__ void __launch_bounds__(256) kv_append_any_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
+__global__ void __launch_bounds__(256) kv_append_any_kernel(KvCache c, KvBatch b, KvNew x) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
   KvPiece p;
-  if (!kv_append_piece(c, b, slots, p)) return;
+  if (!kv_append_piece(c, b, p)) return;
   for (; p.piece < 2 * c.kv_heads; p.piece += p.stride) {
     const int part = p.piece >= c.kv_heads, head = p.piece - part * c.kv_heads;
     int8_t *dst = c.block(p.page, part, head, p.in_page);
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) kv_append_any_kernel(KvCache c, KvBatch b
 // bf16 rows through the division: few-bit operands meet the middle often.)  16 x 1024 tokens, 16 heads of
 // 128, bf16: 40 us (4.9 TB/s, 0.76 of a plain copy).
 template <typename T, int D>
-__global__ void __launch_bounds__(256, sizeof(T) * D <= 256 ? 3 : 1) kv_append_kernel(KvCache c, KvBatch b, KvNew x, int slots) {
+__global__ void __launch_bounds__(256, sizeof(T) * D <= 256 ? 3 : 1) kv_append_kernel(KvCache c, KvBatch b, KvNew x) {
   constexpr int E = 16 / sizeof(T);          // elements of an access
   constexpr int LPR = D / E < 32 ? D / E : 32;  // lanes of a row
   constexpr int RPP = 32 / LPR;              // rows of a pass
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(256, sizeof(T) * D <= 256 ? 3 : 1) kv_append_k
   pdl_trigger();
   const int lane = threadIdx.x & 31;
   KvPiece p;
-  if (!kv_append_piece(c, b, slots, p)) return;
+  if (!kv_append_piece(c, b, p)) return;
   const int r0 = lane / LPR, col = lane % LPR * E;
   const auto element = [](const uint4 &u, int e) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -562,7 +562,7 @@ extern "C" int rt_kv_append(void *codes, float *scales, int64_t n_pages, int64_t
   // (an fp32 block of width 256 does not fit a warp's registers)
   const auto kernel = [&](auto *any, auto *d32, auto *d64, auto *d128, auto *d256) {
     auto *f = !vec ? any : padded_dim == 32 ? d32 : padded_dim == 64 ? d64 : padded_dim == 128 ? d128 : d256;
-    launch_k(f, grid, 256, 0, as_stream(stream), c, b, x, static_cast<int>(slots));
+    launch_k(f, grid, 256, 0, as_stream(stream), c, b, x);
   };
   if (dtype == RT_F32)
     kernel(kv_append_any_kernel<float>, kv_append_kernel<float, 32>, kv_append_kernel<float, 64>,

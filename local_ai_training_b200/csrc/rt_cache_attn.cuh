@@ -270,12 +270,12 @@ struct KaShape {
   static constexpr int VCH = D >= 128 ? D / 128 : 1;     // V chunks of a key per lane
   static constexpr int VB = D >= 128 ? 16 : D / 8;       // their bytes
   static constexpr int STAGE = 2 * 16 * D + 16;          // bytes of a stage of one warp, scales last
-  static constexpr int STAGES = D >= 256 || (D == 128 && NT == 1 && !F32) ? 2 : 4;
+  static constexpr int STAGES = D >= 256 ? 2 : 4;
   static constexpr int RING = KA_WARPS * STAGES * STAGE;
   static constexpr int OP = D + 4;                       // floats of a merged row
   static constexpr int MERGE = KA_WARPS * RT * (OP + 2) * 4;
   static constexpr int SMEM = RING + MERGE;
-  static constexpr int MIN_CTAS = NT == 1 && D <= 128 && !F32 ? 2 : 1;
+  static constexpr int MIN_CTAS = NT == 1 && D <= 64 && !F32 ? 2 : 1;
 };
 
 template <typename T, int D, int NT>
@@ -593,73 +593,119 @@ __global__ void __launch_bounds__(KA_WARPS * 32, KaShape<T, D, NT>::MIN_CTAS)
 
 // Joins the partial rows of every unit that a CTA began and did not end: its own, then those of the
 // following CTAs up to the one that ended the unit, in that order.  A warp takes a row at a time (grid.y
-// CTAs share a unit's rows); lanes over the partials for the factors, then over the width.
+// CTAs share a unit's rows), lanes over the width.  Up to four partials are taken at once, every lane with all
+// their factors; of more (a long sequence over much of the GPU) the lanes share the factors out.  (That form for
+// any number took 280 instructions a row: 22 us for the units of 148 CTAs, 256 rows of 128 each.)
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(KvCache c, KvBatch bt, KvAttn a, int ctas) {
   constexpr int W = D >= 128 ? 4 : D / 32, CH = D / (32 * W);  // floats of a lane's access, accesses
+  constexpr int FEW = 4;
   pdl_wait();
   pdl_trigger();
-  const int4 mt = a.meta[blockIdx.x];
+  const int lane = threadIdx.x & 31, first = blockIdx.x;
+  int4 mt = a.meta[min(first + lane, ctas - 1)];
+  uint32_t ends = __ballot_sync(0xffffffffu, lane > 0 && (first + lane >= ctas - 1 || mt.w != 0));
+  mt.x = __shfl_sync(0xffffffffu, mt.x, 0);
   if (mt.x < 0) return;
-  const int lane = threadIdx.x & 31;
+  mt.y = __shfl_sync(0xffffffffu, mt.y, 0), mt.z = __shfl_sync(0xffffffffu, mt.z, 0);
+  int last = first;  // the CTA that ended the unit
+  while (ends == 0) {
+    last += 32;
+    const int x = last + lane;
+    ends = __ballot_sync(0xffffffffu, x >= ctas - 1 || a.meta[x].w != 0);
+  }
+  last = min(last + __ffs(ends) - 1, ctas - 1);
   const KvSeq q = kv_seq(bt, c.page_size, mt.x);
   const int rows = min(RT, q.n * a.group - mt.y * RT);
-  int last = blockIdx.x + 1;  // the CTA that ended the unit
-  for (;; last += 32) {
-    const int x = last + lane;
-    const uint32_t ends = __ballot_sync(0xffffffffu, x >= ctas - 1 || a.meta[x].w != 0);
-    if (ends != 0) {
-      last = min(last + __ffs(ends) - 1, ctas - 1);
-      break;
+  const int64_t next = static_cast<int64_t>(2 * RT) * (D + 4);  // floats from a CTA's slot to the next one's
+  const auto load = [&](float (&v)[CH * W], const float *p) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      float *to = v + k * W;
+      const float *from = p + 4 + lane * W + k * 128;
+      if constexpr (W == 4)
+        *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(from);
+      else if constexpr (W == 2)
+        *reinterpret_cast<float2 *>(to) = *reinterpret_cast<const float2 *>(from);
+      else
+        *to = *from;
     }
-  }
-  const int first = blockIdx.x;
+  };
 #pragma unroll 1
   for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
-    const int row = mt.y * RT + r;
-    const auto slot = [&](int cta) {
-      return a.ws + (static_cast<int64_t>(cta * 2 + (cta == first)) * RT + r) * (D + 4);
-    };
-    float top = -1e30f;
-    for (int x = first + lane; x <= last; x += 32) top = fmaxf(top, slot(x)[0]);
-    top = warp_max(top);
-    float den = 0.0f, acc[CH * W];
+    // the first CTA's partial is in its second slot, those of the others in their first
+    const float *p0 = a.ws + (static_cast<int64_t>(first * 2 + 1) * RT + r) * (D + 4);
+    const float *pn = p0 + static_cast<int64_t>(RT) * (D + 4);
+    float top = -1e30f, den = 0.0f, acc[CH * W];
+    if (last - first < FEW) {
+      float2 ml[FEW];
+      float v[FEW][CH * W];
 #pragma unroll
-    for (int i = 0; i < CH * W; ++i) acc[i] = 0.0f;
-    for (int x0 = first; x0 <= last; x0 += 32) {
-      float f = 0.0f;
-      if (x0 + lane <= last) {
-        const float2 ml = *reinterpret_cast<const float2 *>(slot(x0 + lane));
-        f = ex2(ml.x - top);
-        den += f * ml.y;
-      }
-      const int n = min(32, last + 1 - x0);
+      for (int i = 0; i < FEW; ++i)
+        if (i <= last - first) {
+          const float *p = i == 0 ? p0 : pn + (i - 1) * next;
+          ml[i] = *reinterpret_cast<const float2 *>(p);
+          load(v[i], p);
+        }
+#pragma unroll
+      for (int i = 0; i < FEW; ++i)
+        if (i <= last - first) top = fmaxf(top, ml[i].x);
+#pragma unroll
+      for (int i = 0; i < CH * W; ++i) acc[i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < FEW; ++i)
+        if (i <= last - first) {
+          const float f = ex2(ml[i].x - top);
+          den += f * ml[i].y;
+#pragma unroll
+          for (int k = 0; k < CH * W; ++k) acc[k] += f * v[i][k];
+        }
+    } else {
+      const auto slot = [&](int cta) { return cta == first ? p0 : pn + (cta - first - 1) * next; };
+      for (int x = first + lane; x <= last; x += 32) top = fmaxf(top, slot(x)[0]);
+      top = warp_max(top);
+#pragma unroll
+      for (int i = 0; i < CH * W; ++i) acc[i] = 0.0f;
+      for (int x0 = first; x0 <= last; x0 += 32) {
+        float f = 0.0f;
+        if (x0 + lane <= last) {
+          const float2 ml = *reinterpret_cast<const float2 *>(slot(x0 + lane));
+          f = ex2(ml.x - top);
+          den += f * ml.y;
+        }
+        const int n = min(32, last + 1 - x0);
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float g = __shfl_sync(0xffffffffu, f, i);
-        const float *p = slot(x0 + i) + 4 + lane * W;
+        for (int i = 0; i < n; ++i) {
+          const float g = __shfl_sync(0xffffffffu, f, i);
+          float v[CH * W];
+          load(v, slot(x0 + i));
 #pragma unroll
-        for (int k = 0; k < CH; ++k) {
-          float v[W];
-          if constexpr (W == 4)
-            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(p + k * 128);
-          else if constexpr (W == 2)
-            *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(p);
-          else
-            v[0] = *p;
-#pragma unroll
-          for (int j = 0; j < W; ++j) acc[k * W + j] += g * v[j];
+          for (int k = 0; k < CH * W; ++k) acc[k] += g * v[k];
         }
       }
+      den = warp_sum_butterfly(den);
     }
-    den = warp_sum_butterfly(den);
     const float inv = den == 0.0f ? 0.0f : __fdividef(1.0f, den);
-    T *o = static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(row / a.group)) * a.o_token +
-           static_cast<int64_t>(mt.z * a.group + row % a.group) * a.o_head;
+    int token, sub;
+    kv_row(a, mt.y * RT + r, token, sub);
+    T *o = static_cast<T *>(a.out) + (q.c0 + static_cast<int64_t>(token)) * a.o_token +
+           static_cast<int64_t>(mt.z * a.group + sub) * a.o_head;
 #pragma unroll
-    for (int i = 0; i < CH * W; ++i) {
-      const int d = (i / W) * 128 + lane * W + i % W;
-      if (d < a.head_dim) store_from_float(o + d, acc[i] * inv);
+    for (int k = 0; k < CH; ++k) {
+      const int d = k * 128 + lane * W;
+      float x[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) x[i] = acc[k * W + i] * inv;
+      if (W == 4 && a.o_vec) {
+        if constexpr (W == 4 && sizeof(T) == 4)
+          *reinterpret_cast<float4 *>(o + d) = make_float4(x[0], x[1], x[2], x[3]);
+        else if constexpr (W == 4)
+          *reinterpret_cast<uint2 *>(o + d) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          if (d + i < a.head_dim) store_from_float(o + d + i, x[i]);
+      }
     }
   }
 }
