@@ -113,12 +113,13 @@ __device__ __forceinline__ void kv_row(const KvAttn &a, int row, int &token, int
 }
 
 // Walks the line of (sequence, row tile, kv head) units from a CTA's first block on.  A unit is RT
-// query rows (token-major, the group's heads innermost) and the blocks of KEYS keys that they see.
-template <int RT, int KEYS>
+// query rows (token-major, the group's heads innermost) and the blocks of KEYS keys that they see.  On the line
+// PAD blocks of no keys stand before each unit, for what its beginning and end take next to a block.
+template <int RT, int KEYS, int PAD = 0>
 struct KvWalk {
   int s, tile, head;       // unit
   int b, e, nb;            // piece [b, e) of the unit's nb blocks
-  int left;                // blocks of the CTA from b on
+  int left;                // length of the CTA's share of the line from b on
   KvSeq q;
   int tiles;
 
@@ -143,13 +144,13 @@ struct KvWalk {
 #pragma unroll 1
     for (tile = 0; tile < tiles; ++tile) {
       set_tile(a);
-      sum += nb;
+      sum += PAD + nb;
     }
     return sum;
   }
-  // the unit after this one (none: left = 0)
+  // the unit after this one (none: left <= 0)
   __device__ __forceinline__ void next(const KvCache &c, const KvBatch &bt, const KvAttn &a) {
-    left -= e - b;
+    left -= e - b + PAD;
     if (left <= 0) return;
     if (++head == c.kv_heads) {
       head = 0;
@@ -173,8 +174,8 @@ struct KvWalk {
 // Sets this CTA's share of the line: all of the grid has equal shares of a long line, and as many CTAs as
 // get min_blocks each of a short one; `used`: the batch's rows.  With min_blocks = 0 a CTA takes one whole unit (the grid has one
 // for each), so no rows are left to join.  Returns false (for every thread) when this CTA has no share.
-template <int THREADS, int RT, int KEYS>
-__device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache &c, const KvBatch &bt,
+template <int THREADS, int RT, int KEYS, int PAD>
+__device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS, PAD> &w, const KvCache &c, const KvBatch &bt,
                                               const KvAttn &a, int min_blocks, int &used) {
   constexpr int WARPS = THREADS / 32;
   __shared__ int sm_sum[WARPS], sm_start[10];
@@ -225,17 +226,18 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
 #pragma unroll 1
       for (w.tile = 0;; ++w.tile) {
         w.set_tile(a);
-        per_head = units ? 1 : w.nb;
+        per_head = units ? 1 : PAD + w.nb;
         if (p0 < at + per_head * c.kv_heads || w.tile >= w.tiles - 1) break;
         at += per_head * c.kv_heads;
       }
       sm_start[0] = w.s, sm_start[1] = w.tile, sm_start[2] = (p0 - at) / per_head;
-      sm_start[3] = p0 - at - sm_start[2] * per_head, sm_start[4] = units ? w.nb : p1 - p0;
+      const int in_unit = p0 - at - sm_start[2] * per_head;
+      sm_start[3] = max(in_unit - PAD, 0), sm_start[4] = units ? w.nb : p1 - p0 - max(PAD - in_unit, 0);
       sm_start[5] = w.q.c0, sm_start[6] = w.q.n, sm_start[7] = w.q.len, sm_start[8] = w.tiles;
     }
   }
   __syncthreads();
-  if (sm_start[0] < 0) return false;
+  if (sm_start[0] < 0 || sm_start[4] <= 0) return false;
   w.s = sm_start[0], w.tile = sm_start[1], w.head = sm_start[2], w.b = sm_start[3];
   w.left = sm_start[4];
   w.q = KvSeq{sm_start[5], sm_start[6], sm_start[7], sm_start[7] - sm_start[6]};
@@ -243,6 +245,16 @@ __device__ __forceinline__ bool kv_walk_start(KvWalk<RT, KEYS> &w, const KvCache
   w.set_tile(a);
   w.e = min(w.nb, w.b + w.left);
   return true;
+}
+
+// Blocks of the CTA's share, the padding not counted.  (Telling the last piece as it comes, instead of counting
+// ahead, cost the many-row kernel's loops 2 % on a long unit.)
+template <int RT, int KEYS, int PAD>
+__device__ __forceinline__ uint32_t kv_walk_blocks(const KvCache &c, const KvBatch &bt, const KvAttn &a,
+                                                   KvWalk<RT, KEYS, PAD> w) {
+  uint32_t n = 0;
+  for (; w.left > 0; w.next(c, bt, a)) n += static_cast<uint32_t>(w.e - w.b);
+  return n;
 }
 
 // Zeros for the rows that belong to no sequence (from cu[n_seqs] = used on).

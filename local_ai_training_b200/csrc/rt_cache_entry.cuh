@@ -114,7 +114,7 @@ int kv_prefill_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms
   static bool done[64] = {false};
   auto *kernel = kv_prefill_kernel<D>;
   if (int rc = kv_allow_smem(kernel, SH::SMEM, mu, done)) return rc;
-  launch_k(kernel, sms, SH::THREADS, SH::SMEM, s, c, bt, a, 2);
+  launch_k(kernel, sms, SH::THREADS, SH::SMEM, s, c, bt, a, KP_PAD + 2);
   launch_k(kv_attention_join_kernel<__nv_bfloat16, D, SH::RT>, dim3(sms, 16), 256, 0, s, c, bt, a, sms);
   return check_launch("kv_attention");
 }
@@ -178,9 +178,10 @@ extern "C" int rt_kv_attention(const void *q, int dtype, int64_t q_stride_token,
   if (q == nullptr || out == nullptr)
     return fail(RT_ERR_INVALID_ARGUMENT, "kv_attention: null pointer");
   if (n_tokens * q_heads > INT32_MAX - 64) return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
-  // the line of (row tile, kv head, key block) fits 31 bits: tiles of 4 rows and blocks of 16 keys at least
+  // the line of (row tile, kv head, key block) fits 31 bits: tiles of 4 rows and blocks of 16 keys at least,
+  // a unit's padding with them
   const int64_t tiles = n_tokens * (q_heads / kv_heads) / 4 + std::min(n_seqs, n_tokens);
-  if (static_cast<double>(tiles) * kv_heads * (pages_per_seq * page_size / KV_BLOCK + 1) > 2e9)
+  if (static_cast<double>(tiles) * kv_heads * (pages_per_seq * page_size / KV_BLOCK + 3) > 2e9)
     return fail(RT_ERR_UNSUPPORTED, "kv_attention: batch too large");
   const int sms = kv_sm_count();
   if (sms <= 0) return fail(RT_ERR_CUDA, "kv_attention: no device");
