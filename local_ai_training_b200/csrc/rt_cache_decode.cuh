@@ -60,6 +60,11 @@ __device__ __forceinline__ float small_int(uint32_t v) {
   return __int_as_float(static_cast<int>(v) + 0x4B400000) - 12582912.0f;
 }
 
+// A unit counts one tile more than it has on the line of work, for its queries in and its results out: 32 sequences
+// of up to 4096 tokens, four each, 32 heads over 8: 71.0 us without and 69.6 so (70.0 with two); 64 of up to 1024,
+// one each, 16 heads: 44.3 and 43.9; long ones alike.
+constexpr int KD_PAD = 1;
+
 template <typename T, int RT>
 struct KdShape {
   static constexpr bool F32 = sizeof(T) == 4;
@@ -144,7 +149,7 @@ template <typename T, int RT>
 __global__ void __launch_bounds__(KdShape<T, RT>::THREADS, 2)
     kv_decode_kernel(const __grid_constant__ CUtensorMap map, KvCache c, KvBatch bt, KvAttn a, int min_blocks) {
   using SH = KdShape<T, RT>;
-  using Walk = KvWalk<RT, SH::KEYS>;
+  using Walk = KvWalk<RT, SH::KEYS, KD_PAD>;
   constexpr int ND = SH::ND, N = SH::N, D = SH::D, RW = SH::RW, W4 = 4 * SH::GROUPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(KdShape<T, RT>::THREADS, 2)
     // ================================================================ MMA issue
     if (lane == 0) {
       const uint64_t q0 = make_sw128_desc(smem_u32(smem + SH::Q_OFF), 16, 1024);
-      const uint32_t total = static_cast<uint32_t>(w.left);  // tiles of this CTA
+      const uint32_t total = kv_walk_blocks(c, bt, a, w);  // tiles of this CTA
       uint32_t n = 0, pieces = 0;
       bool ok = true;
       const auto scores = [&](uint32_t i) {

@@ -103,7 +103,7 @@ int kv_decode_run(const KvCache &c, const KvBatch &bt, const KvAttn &a, int sms,
     launch_k(kernel, static_cast<unsigned>(units), SH::THREADS, SH::SMEM, s, map, c, bt, a, 0);
     return check_launch("kv_attention");
   }
-  launch_k(kernel, ctas, SH::THREADS, SH::SMEM, s, map, c, bt, a, 2);
+  launch_k(kernel, ctas, SH::THREADS, SH::SMEM, s, map, c, bt, a, KD_PAD + 2);
   launch_k(kv_attention_join_kernel<T, 128, RT>, dim3(ctas, (RT + 7) / 8), 256, 0, s, c, bt, a, ctas);
   return check_launch("kv_attention");
 }
