@@ -12,9 +12,9 @@
 //   O^T [128 dims x N] = V^T (the tile as it lies, M-major) · P^T (N rows of digits over the keys)
 // Products and sums are exact (|sum| < 2^21); a thread is a key in S^T and a dim in O^T, so it holds all
 // digits of its rows and joins them in fp32.  O is summed in registers, rescaled as m moves.
-// Measured: 16 sequences of up to 32768 tokens, 8 shared heads, 122 us (6.0 TB/s, 0.92 of a plain copy);
-// 64 of up to 1024, 16 heads, 45 us (4.5 TB/s: some 5 us of start, and pieces of 8 tiles); 16 rows per head
-// (four drafted tokens, four query heads), 32 x 4096 tokens, 73 us (2.9 TB/s: bound by the softmax of 16 rows).
+// Measured: 16 sequences of up to 32768 tokens, 8 shared heads, 121 us (6.1 TB/s, 0.93 of a plain copy);
+// 64 of up to 1024, 16 heads, 44 us (4.6 TB/s: some 5 us of start, and pieces of 8 tiles); 16 rows per head
+// (four drafted tokens, four query heads), 32 x 4096 tokens, 70 us (3.0 TB/s: bound by the softmax of 16 rows).
 //   warps 0-3 (0-7 for 16 rows: eight rows each)  scores -> weights -> digits; sums of O, a tile behind, while the tensor core works
 //   the next warp  TMA: page entries, tiles of 128 keys of K and V, block scales
 //   the last warp  one thread issues the products, the next tile's scores before this one's outputs

@@ -15,8 +15,8 @@
 // The block scales are folded into the scores and the weights (a factor per 16 keys).  The weight
 // 2^(t - m)·sv is rounded to bf16 (bf16 queries only; the sum of weights keeps 32 bits).  The running
 // maximum moves, and O is rescaled, only when a score exceeds it by 2^8.
-// Measured: a piece of 2048 tokens over 32768, 32 heads over 8 of 128, 1.41 ms (0.80 PFLOP/s, 0.48 of the cuBLAS
-// bf16 rate); eight prompts of up to 1024 tokens, 16 heads, 112 us.  A step takes 5.6 k cycles instead of
+// Measured: a piece of 2048 tokens over 32768, 32 heads over 8 of 128, 1.42 ms (0.80 PFLOP/s, 0.48 of the cuBLAS
+// bf16 rate); eight prompts of up to 1024 tokens, 16 heads, 94 us.  A step takes 5.6 k cycles instead of
 // 2.0 k: a row tile's softmax (some 3.5 k cycles of dependent loads, votes and exponentials) is longer
 // than the other's products, and the products share the bandwidth of shared memory with the
 // conversion of the next tile.  Loops are kept rolled: unrolled bodies missed the instruction cache

@@ -284,6 +284,20 @@ def test_attention_rows_around_the_tiles(cuda_device, rows, dim):
     assert _status(cuda_device) == 0
 
 
+@pytest.mark.parametrize("seqs", [1, 2, 5, 37, 150])
+@pytest.mark.parametrize("new", [1, 3, 100])
+def test_attention_shares_that_end_anywhere_in_short_units(cuda_device, seqs, new):
+    """Units of one to seven blocks, from fewer than the GPU has places to many for each: the shares of the line
+    of work end before, at the beginning of, in and behind units."""
+    lens = [(137 * i) % 770 + 130 for i in range(seqs)]
+    case = _Case(cuda_device, lens, [new] * seqs, heads=6, kv_heads=3, dim=128, page=32, seed=seqs)
+    q = case.queries(torch.bfloat16)
+    got = case.run(q)
+    case.check(got, q)
+    assert torch.equal(case.run(q), got)
+    assert _status(cuda_device) == 0
+
+
 def test_attention_bad_pages_and_lengths_are_flagged(cuda_device):
     case = _Case(cuda_device, [60, 60], [1, 1])
     q = case.queries(torch.bfloat16)
