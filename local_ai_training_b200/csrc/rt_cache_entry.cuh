@@ -13,8 +13,8 @@ inline int kv_sm_count() {
 }
 constexpr int KA_GRID = 2;       // CTAs per SM of the few-row kernel, at most
 // Rows per kv head from which a sequence takes the many-row kernel.  One sequence of 8192 tokens, 8 kv heads:
-// 27 us by the few-row kernel and 30 by this one at 64 rows, 39 and 33 at 128; eight of 4096 tokens: 63 and
-// 64 us at 64 rows, 115 and 69 at 128.
+// 26 us by the few-row kernel and 30 by this one at 64 rows, 38 and 31 at 128; eight of 4096 tokens: 70 and
+// 64 us at 64 rows, 121 and 66 at 128.
 constexpr int KP_MIN_ROWS = 96;
 
 // Whether a sequence of the batch may take the tcgen05 kernel: one that has the batch to itself, or all
@@ -51,7 +51,7 @@ inline int64_t kv_most_tiles(int64_t n_seqs, int64_t n_tokens, int64_t group, in
   return group <= tile ? std::min(tiles, n_tokens) : tiles;
 }
 // Rows of a tile of the few-row kernels, by the rows that the sequences average per kv head.  Heads of 128, 32
-// sequences of 2048 tokens, 16 kv heads: 52 us in tiles of 4 and 69 in tiles of 16 for 4 rows, 92 and 71 for
+// sequences of 2048 tokens, 16 kv heads: 60 us in tiles of 4 and 78 in tiles of 16 for 4 rows, 97 and 80 for
 // 6; heads of 64, 16 sequences, 8 heads: 22 us in tiles of 8 and 26 of 16 for 8 rows, 32 and 28 for 12.
 inline int kv_tile(int64_t n_seqs, int64_t n_tokens, int64_t group, int64_t dim) {
   const int64_t rows = n_tokens * group;
@@ -59,7 +59,7 @@ inline int kv_tile(int64_t n_seqs, int64_t n_tokens, int64_t group, int64_t dim)
   return dim < 128 && rows > 8 * n_seqs ? 16 : 8;
 }
 // Short units, up to two waves of them, take one CTA each and no join: 16 sequences of 512 tokens, 16 heads of
-// 128, 9.1 us so and 14.2 with the line cut, 32 of them 16.8 and 18.4, one 7.6 and 9.9; one of 1024 tokens
+// 128, 11.0 us so and 14.9 with the line cut, 32 of them 20.4 and 20.3, one 7.3 and 9.5; one of 1024 tokens
 // 10.5 and 10.1 (8 heads of 64: 11.7 and 9.0).  Returns their number, or 0 when the line is to be cut.
 inline int64_t kv_whole_units(int64_t n_seqs, int64_t n_tokens, int64_t group, int64_t kv_heads, int64_t dim,
                               int64_t room, int dtype, int64_t sms) {
